@@ -1,0 +1,176 @@
+"""Host side of the 8-bit decoder operators: rotary frequencies, argument checks of the C entries, refusals without a GPU."""
+
+import ctypes
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from verdict_b200 import _abi, ops  # noqa: E402
+
+
+def radians(turns):
+    return [2 * math.pi * t / 2.0 ** 64 for t in turns]
+
+
+def plain(rd, theta):
+    return [theta ** (-2.0 * i / rd) for i in range(rd // 2)]
+
+
+def close(got, want):
+    for g, w in zip(got, want):
+        # whole turns drop out; a double's 53 bits on a frequency of at most one radian
+        assert abs(math.remainder(g - w, 2 * math.pi)) <= 2.0 ** -50, (g, w)
+
+
+def test_rotary_turns_plain_and_linear():
+    for rd, theta in ((2, 1e4), (64, 1e4), (128, 1e6)):
+        t, m = ops.rotary_turns(rd, theta)
+        assert m == 1.0 and len(t) == rd // 2
+        close(radians(t), plain(rd, theta))
+        t, m = ops.rotary_turns(rd, theta, {"type": "linear", "factor": 4.0})
+        close(radians(t), [f / 4 for f in plain(rd, theta)])
+
+
+def test_rotary_turns_ntk():
+    t, _ = ops.rotary_turns(64, 1e4, {"type": "ntk", "factor": 8.0})
+    close(radians(t), plain(64, 1e4 * 8.0 ** (64 / 62)))
+    # The slowest pair ends up divided by the factor, the fastest as it was.
+    close(radians(t)[-1:], [plain(64, 1e4)[-1] / 8])
+
+
+def test_rotary_turns_yarn_matches_a_worked_ramp():
+    rd, theta, orig, factor = 128, 1e6, 32768, 4.0
+    t, m = ops.rotary_turns(rd, theta, {"type": "yarn", "factor": factor, "original_max_position": orig})
+    assert m == pytest.approx(0.1 * math.log(4) + 1, rel=1e-7)
+    f = plain(rd, theta)
+    turns_in_context = [x * orig / (2 * math.pi) for x in f]
+    got = radians(t)
+    for i in range(rd // 2):
+        if turns_in_context[i] > 40:
+            close([got[i]], [f[i]])
+        elif turns_in_context[i] < 0.9:
+            close([got[i]], [f[i] / factor])
+        else:
+            assert f[i] / factor * (1 - 1e-12) <= got[i] <= f[i] * (1 + 1e-12)
+    assert all(a >= b for a, b in zip(got, got[1:]))
+    _, m = ops.rotary_turns(rd, theta, {"type": "yarn", "factor": 4.0, "original_max_position": orig,
+                                        "attention_factor": 1.25})
+    assert m == 1.25
+
+
+def test_rotary_turns_llama3_bands():
+    rd, theta, orig, factor = 128, 5e5, 8192, 8.0
+    t, m = ops.rotary_turns(rd, theta, {"type": "llama3", "factor": factor, "original_max_position": orig,
+                                        "low_freq_factor": 1.0, "high_freq_factor": 4.0})
+    assert m == 1.0
+    for got, f in zip(radians(t), plain(rd, theta)):
+        wave = 2 * math.pi / f
+        if wave < orig / 4:
+            want = f
+        elif wave > orig:
+            want = f / factor
+        else:
+            s = (orig / wave - 1) / 3
+            want = (1 - s) * f / factor + s * f
+        close([got], [want])
+
+
+def test_rotary_turns_divisors():
+    d = [1.0 + i for i in range(8)]
+    t, m = ops.rotary_turns(16, 1e4, {"type": "divisors", "divisors": d, "attention_factor": 1.5})
+    assert m == 1.5
+    close(radians(t), [f / x for f, x in zip(plain(16, 1e4), d)])
+
+
+@pytest.mark.parametrize("rd,scaling", [
+    (3, None), (0, None), (2048, None), (64, {"type": "cubic"}), (64, {"type": "linear"}),
+    (64, {"type": "linear", "factor": 2.0, "extra": 1}), (64, {"type": "divisors", "divisors": [1.0]})])
+def test_rotary_turns_refusals(rd, scaling):
+    with pytest.raises(ValueError):
+        ops.rotary_turns(rd, 1e4, scaling)
+
+
+@pytest.mark.parametrize("theta,scaling", [
+    (0.0, None), (math.nan, None), (1e4, {"type": "linear", "factor": 0.5}),
+    (1e4, {"type": "yarn", "factor": 2.0, "original_max_position": 0}),
+    (1e4, {"type": "llama3", "factor": 2.0, "original_max_position": 8, "low_freq_factor": 4.0, "high_freq_factor": 1.0}),
+    (1e4, {"type": "divisors", "divisors": [0.0] * 32})])
+def test_rotary_turns_values_refused_by_the_library(theta, scaling):
+    with pytest.raises(_abi.VdError) as e:
+        ops.rotary_turns(64, theta, scaling)
+    assert e.value.code == _abi.VD_EINVAL
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x = torch.zeros(2, 128)
+    for f in (lambda: ops.quantize_fp8(x), lambda: ops.quantize_fp8_weight(x), lambda: ops.block_norm(x, x),
+              lambda: ops.token_logprobs(x), lambda: ops.quantize_fp8("x")):
+        with pytest.raises(ValueError):
+            f()
+
+
+def call(name, *args):
+    err = ctypes.create_string_buffer(512)
+    rc = getattr(_abi.load(), name)(*args, None, err, 512)
+    return rc, err.value.decode()
+
+
+FAKE = 1 << 20  # an address that no check reads
+
+
+def test_c_entries_check_before_they_launch():
+    """Bad arguments come back as VD_EINVAL with a message; zero rows are no work.  No device is needed for either."""
+    E = _abi.VD_EINVAL
+    cases = [
+        ("vdk_quantize_fp8", (FAKE, 128, None, 0, 0, -1, 128, 0, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8", (FAKE, 100, None, 0, 0, 2, 128, 0, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8", (FAKE, 128, None, 0, 4, 2, 128, 0, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8", (None, 128, None, 0, 0, 2, 128, 0, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8", (FAKE, 128, None, 0, 0, 2, 128, 7, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8", (FAKE, 128, None, 0, 0, 1 << 40, 128, 0, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8_weight", (FAKE, 128, 0, 128, 0, FAKE, 128, FAKE, 1)),
+        ("vdk_quantize_fp8_weight", (FAKE, 128, 4, 128, 9, FAKE, 128, FAKE, 1)),
+        ("vdk_fp8_linear", (FAKE, 128, FAKE, 1, FAKE, 128, FAKE, 1, 4, 4, 0, None, FAKE, 4, 0, None)),
+        ("vdk_fp8_linear", (FAKE + 8, 128, FAKE, 1, FAKE, 128, FAKE, 1, 4, 4, 128, None, FAKE, 4, 0, None)),
+        ("vdk_fp8_linear", (FAKE, 136, FAKE, 1, FAKE, 128, FAKE, 1, 4, 4, 128, None, FAKE, 4, 0, None)),
+        ("vdk_fp8_linear", (FAKE, 128, FAKE, 0, FAKE, 128, FAKE, 1, 4, 4, 128, None, FAKE, 4, 0, None)),
+        ("vdk_fp8_linear", (FAKE, 128, FAKE, 1, FAKE, 128, FAKE, 1, 4, 4, 128, None, FAKE, 3, 0, None)),
+        ("vdk_fp8_linear", (FAKE, 128, FAKE, 1, FAKE, 128, FAKE, 1, 4, 4, 128, None, FAKE, 4, 3, None)),
+        ("vdk_block_norm", (FAKE, 8, 0, FAKE, 8, 1, None, None, 0, 0, 0, 1.0, 1.0, None, 1e-6, 0, 2, 8, FAKE, 8, None, 0,
+                            0, None, 0)),
+        ("vdk_block_norm", (FAKE, 8, 0, FAKE, 8, 2, None, None, 0, 0, 0, 1.0, 1.0, None, 1e-6, 0, 2, 8, None, 8, None, 0,
+                            0, None, 0)),
+        ("vdk_block_norm", (FAKE, 8, 0, FAKE, 8, 2, None, FAKE, 2, 8, 2, 1.0, 1.0, None, 1e-6, 0, 2, 8, FAKE, 8, None, 0,
+                            0, None, 0)),
+        ("vdk_block_norm", (FAKE, 8, 0, FAKE, 8, 2, None, None, 0, 0, 0, 1.0, 1.0, FAKE, 1e-6, 0, 2, 8, FAKE, 8, FAKE, 8,
+                            3, None, 0)),
+        ("vdk_block_norm", (FAKE, 20000, 0, None, 0, 2, None, None, 0, 0, 0, 1.0, 1.0, None, 1e-6, 0, 2, 20000, FAKE,
+                            20000, None, 0, 0, None, 0)),
+        ("vdk_rotary", (None, None, 2, 64, 64, 0, 0, 0, None, 0, 0, FAKE, 1.0)),
+        ("vdk_rotary", (_abi.VdkRotaryHeads(FAKE, FAKE, 64, 64, 64, 0, 2), None, 2, 64, 64, 0, 0, 0, None, 0, 0, FAKE, 1.0)),
+        ("vdk_rotary", (_abi.VdkRotaryHeads(FAKE, FAKE, 64, 64, 64, 64, 1), None, 2, 64, 65, 0, 0, 0, None, 0, 0, FAKE, 1.0)),
+        ("vdk_rotary", (_abi.VdkRotaryHeads(FAKE, FAKE, 64, 64, 64, 64, 1), None, 2, 64, 64, 0, 0, 0, FAKE, 16, 0, FAKE, 1.0)),
+        ("vdk_rotary", (_abi.VdkRotaryHeads(FAKE, FAKE, 64, 64, 64, 64, 1), None, 2, 64, 64, 0, 0, 0, None, 0, 0, None, 1.0)),
+        ("vdk_token_logprobs", (FAKE, 10, 2, 20, 0, 1.0, None, 0, 0, None, None, None, None, None)),
+        ("vdk_token_logprobs", (FAKE, 20, 2, 20, 0, 0.0, None, 0, 0, None, None, None, None, None)),
+        ("vdk_token_logprobs", (FAKE, 20, 2, 20, 0, 1.0, None, 0, 65, None, None, None, FAKE, FAKE)),
+        ("vdk_token_logprobs", (FAKE, 20, 2, 20, 0, 1.0, None, 2, 0, FAKE, None, None, None, None)),
+        ("vdk_token_logprobs", (FAKE, 20, 2, 20, 0, 1.0, None, 0, 3, None, None, None, None, FAKE)),
+    ]
+    for name, args in cases:
+        rc, msg = call(name, *args)
+        assert rc == E and msg, (name, args, rc, msg)
+    nothing = [
+        ("vdk_quantize_fp8", (None, 128, None, 0, 0, 0, 128, 0, None, 128, None, 1)),
+        ("vdk_fp8_linear", (None, 128, None, 1, FAKE, 128, FAKE, 1, 0, 4, 128, None, None, 4, 0, None)),
+        ("vdk_block_norm", (None, 8, 0, None, 8, 2, None, None, 0, 0, 0, 1.0, 1.0, None, 1e-6, 0, 0, 8, None, 8, None, 0,
+                            0, None, 0)),
+        ("vdk_token_logprobs", (None, 20, 0, 20, 0, 1.0, None, 0, 0, None, None, None, None, None)),
+    ]
+    for name, args in nothing:
+        assert call(name, *args)[0] == _abi.VD_OK, name
+    # A null error buffer is allowed.
+    assert _abi.load().vdk_token_logprobs(FAKE, 10, 2, 20, 0, 1.0, None, 0, 0, None, None, None, None, None, None, None,
+                                          0) == E

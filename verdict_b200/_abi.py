@@ -14,9 +14,11 @@ from . import build as _build
 
 VD_OK, VD_EINVAL, VD_ECUDA, VD_EDEAD, VD_ENOMEM, VD_ESPEC, VD_EDEVICE = 0, -1, -2, -3, -4, -5, -6
 VD_MEM_HOST, VD_MEM_DEVICE = 0, 1
-VDK_FP16, VDK_BF16 = 0, 1
+VDK_FP16, VDK_BF16, VDK_FP32, VDK_FP8 = 0, 1, 2, 3
 
 _P = ctypes.c_void_p
+_I64, _INT, _F32 = ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_STR, _SIZE = ctypes.c_char_p, ctypes.c_size_t
 _I64P = ctypes.POINTER(ctypes.c_int64)
 
 
@@ -40,6 +42,15 @@ class VdStats(ctypes.Structure):
         ("fork_groups", ctypes.c_int64), ("fork_rows", ctypes.c_int64), ("shared_tokens", ctypes.c_int64),
         ("prep_ms", ctypes.c_double), ("finish_ms", ctypes.c_double), ("upload_ms", ctypes.c_double),
         ("download_ms", ctypes.c_double),
+    ]
+
+
+class VdkRotaryHeads(ctypes.Structure):
+    _fields_ = [
+        ("input", _P), ("output", _P),
+        ("in_token", ctypes.c_int64), ("in_head", ctypes.c_int64),
+        ("out_token", ctypes.c_int64), ("out_head", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
     ]
 
 
@@ -82,6 +93,18 @@ SIGNATURES = {
                                              ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P,
                                              ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_char_p,
                                              ctypes.c_size_t]),
+    "vdk_quantize_fp8": (ctypes.c_int, [_P, _I64, _P, _I64, _INT, _I64, _I64, _INT, _P, _I64, _P, _I64, _P, _STR,
+                                        _SIZE]),
+    "vdk_quantize_fp8_weight": (ctypes.c_int, [_P, _I64, _I64, _I64, _INT, _P, _I64, _P, _I64, _P, _STR, _SIZE]),
+    "vdk_fp8_linear": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _INT, _P,
+                                      _P, _STR, _SIZE]),
+    "vdk_block_norm": (ctypes.c_int, [_P, _I64, _INT, _P, _I64, _INT, _P, _P, _INT, _I64, _I64, _F32, _F32, _P, _F32,
+                                      _INT, _I64, _I64, _P, _I64, _P, _I64, _INT, _P, _I64, _P, _STR, _SIZE]),
+    "vdk_rotary_turns": (ctypes.c_int, [ctypes.c_double, _INT, _INT, _P, _P, _P, _P, _STR, _SIZE]),
+    "vdk_rotary": (ctypes.c_int, [ctypes.POINTER(VdkRotaryHeads), ctypes.POINTER(VdkRotaryHeads), _I64, _INT, _INT,
+                                  _INT, _INT, _INT, _P, _INT, _I64, _P, _F32, _P, _STR, _SIZE]),
+    "vdk_token_logprobs": (ctypes.c_int, [_P, _I64, _I64, _I64, _INT, _F32, _P, _I64, _INT, _P, _P, _P, _P, _P, _P,
+                                          _STR, _SIZE]),
 }
 
 _lib = None

@@ -1,0 +1,435 @@
+// C entry points of the 8-bit decoder operators (include/vdexec_kernels.h):
+// argument checks, the choice of a kernel variant and the launch on the
+// caller's stream.  Nothing here allocates or waits.
+
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "vdexec_kernels.h"
+
+#include "block_norm.cuh"
+#include "fp8_gemm.cuh"
+#include "host.hpp"
+#include "quantize.cuh"
+#include "rotary.cuh"
+#include "token_logprobs.cuh"
+
+namespace vd {
+namespace {
+
+constexpr int64_t kMaxInt = 0x7fffffff;
+
+void need(bool ok, const char* what) {
+  if (!ok) fail(VD_EINVAL, what);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int elem_bytes(int dtype) { return dtype == VDK_FP32 ? 4 : 2; }
+
+// Rows of `dtype` that all start on a 16-byte boundary.
+bool rows16(const void* p, int64_t ld, int dtype) { return aligned16(p) && ld * elem_bytes(dtype) % 16 == 0; }
+
+template <class F>
+void by_type(int dtype, F&& f) {
+  switch (dtype) {
+    case VDK_FP16: f(__half()); break;
+    case VDK_BF16: f(__nv_bfloat16()); break;
+    case VDK_FP32: f(float()); break;
+    default: fail(VD_EINVAL, "dtype must be VDK_FP16, VDK_BF16 or VDK_FP32");
+  }
+}
+
+int sm_count() {
+  static int sms[64] = {};
+  int dev = 0;
+  cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (dev < 0 || dev >= 64) fail(VD_EINVAL, "device index out of range");
+  if (!sms[dev]) {  // the same value whichever thread stores it
+    int n = 0;
+    cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+void launched() { cuda_check(cudaGetLastError(), "kernel launch"); }
+
+template <class K, class... Args>
+void launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                    const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), "kernel launch");
+}
+
+// Row-major [rows, cols] bytes with row stride ld, boxes of box_rows x 128
+// with the 128-byte swizzle; columns and rows past the end read as zero.
+CUtensorMap f8_map(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  CUtensorMap m;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(VD_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")");
+  return m;
+}
+
+template <bool SWAP, int BN, class O>
+void launch_f8(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8Shape s, int* status, cudaStream_t stream) {
+  using Cfg = F8Config<BN>;
+  auto kernel = fp8_gemm_kernel<SWAP, BN, O>;
+  cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES),
+             "shared memory size");
+  const CUtensorMap ma = f8_map(a, s.M, s.K, ld_a, SWAP ? BN : 128);
+  const CUtensorMap mw = f8_map(w, s.N, s.K, ld_w, SWAP ? 128 : BN);
+  const int p_tiles = ((SWAP ? s.N : s.M) + 127) / 128;
+  const int q_tiles = ((SWAP ? s.M : s.N) + BN - 1) / BN;
+  // K is split while the CTAs still fit on the GPU at once (one per SM) and
+  // each keeps at least four k-blocks.
+  const int kblocks = (s.K + 127) / 128;
+  const int tiles = p_tiles * q_tiles;
+  s.splits = 1;
+  while (s.splits < 8 && tiles * (s.splits + 1) <= sm_count() && kblocks / (s.splits + 1) >= 4) ++s.splits;
+  launch_cluster(kernel, dim3(p_tiles * s.splits, q_tiles), Cfg::THREADS, Cfg::SMEM_BYTES, s.splits, stream,
+                 SWAP ? mw : ma, SWAP ? ma : mw, s, status);
+}
+
+}  // namespace
+}  // namespace vd
+
+using namespace vd;
+
+extern "C" VD_API int vdk_quantize_fp8(const void* x, int64_t ld_x, const void* gate, int64_t ld_gate, int act,
+                                       int64_t rows, int64_t cols, int dtype, void* q, int64_t ld_q, float* scale,
+                                       int64_t ld_scale, void* stream, char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(rows >= 0 && cols >= 1 && cols <= kMaxInt - 128, "need rows >= 0 and 1 <= cols < 2^31 - 128");
+    need(act >= VDK_ACT_NONE && act <= VDK_ACT_SILU, "unknown activation");
+    need(gate || act == VDK_ACT_NONE, "an activation needs a gate");
+    const int64_t col_blocks = (cols + 127) / 128;
+    need(rows * col_blocks <= kMaxInt, "rows * ceil(cols / 128) must be below 2^31");
+    need(ld_x >= cols && ld_q >= cols && ld_scale >= col_blocks && (!gate || ld_gate >= cols),
+         "a row stride is smaller than its row");
+    if (rows == 0) return;
+    need(x && q && scale, "null buffer");
+    QuantizeParams p{};
+    p.x = x, p.gate = gate;
+    p.ld_x = ld_x, p.ld_gate = ld_gate, p.ld_q = ld_q, p.ld_scale = ld_scale;
+    p.blocks = static_cast<uint32_t>(rows * col_blocks);
+    p.col_blocks = static_cast<uint32_t>(col_blocks);
+    p.cols = static_cast<int>(cols);
+    p.act = act;
+    p.q = static_cast<uint8_t*>(q);
+    p.scale = scale;
+    p.q_aligned = (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ld_q % 8 == 0;
+    const unsigned per = kQuantUnroll * kQuantThreads / 16;
+    const unsigned grid = (p.blocks + per - 1) / per;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    by_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      const bool al = rows16(x, ld_x, dtype) && (!gate || rows16(gate, ld_gate, dtype));
+      if (gate) {
+        if (al) quantize_rows_kernel<T, true, true><<<grid, kQuantThreads, 0, s>>>(p);
+        else quantize_rows_kernel<T, true, false><<<grid, kQuantThreads, 0, s>>>(p);
+      } else {
+        if (al) quantize_rows_kernel<T, false, true><<<grid, kQuantThreads, 0, s>>>(p);
+        else quantize_rows_kernel<T, false, false><<<grid, kQuantThreads, 0, s>>>(p);
+      }
+    });
+    launched();
+  });
+}
+
+extern "C" VD_API int vdk_quantize_fp8_weight(const void* w, int64_t ld_w, int64_t rows, int64_t cols, int dtype,
+                                              void* q, int64_t ld_q, float* scale, int64_t ld_scale, void* stream,
+                                              char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(rows >= 1 && rows <= 65535ll * 128 && cols >= 1 && cols <= kMaxInt - 128,
+         "need 1 <= rows <= 8388480 and 1 <= cols < 2^31 - 128");
+    need(ld_w >= cols && ld_q >= cols && ld_scale >= (cols + 127) / 128, "a row stride is smaller than its row");
+    need(w && q && scale, "null buffer");
+    const dim3 grid(static_cast<unsigned>((cols + 127) / 128), static_cast<unsigned>((rows + 127) / 128));
+    by_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      quantize_weight_kernel<T><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+          static_cast<const T*>(w), ld_w, static_cast<int>(rows), static_cast<int>(cols), static_cast<uint8_t*>(q), ld_q,
+          scale, ld_scale);
+    });
+    launched();
+  });
+}
+
+extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale,
+                                     const void* w, int64_t ld_w, const float* w_scale, int64_t ld_w_scale, int64_t M,
+                                     int64_t N, int64_t K, const float* bias, void* out, int64_t ld_out, int out_dtype,
+                                     int* status, void* stream, char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(M >= 0 && N >= 1 && K >= 1, "need M >= 0, N >= 1 and K >= 1");
+    need(M <= (int64_t(1) << 30) && N <= 65535ll * 32 && K <= (int64_t(1) << 30), "a dimension is too large");
+    const int64_t kb = (K + 127) / 128;
+    need(ld_a >= K && ld_w >= K && ld_out >= N && ld_a_scale >= kb && ld_w_scale >= kb,
+         "a row stride is smaller than its row");
+    need(out_dtype >= VDK_FP16 && out_dtype <= VDK_FP32, "out_dtype must be VDK_FP16, VDK_BF16 or VDK_FP32");
+    if (M == 0) return;
+    need(a && w && a_scale && w_scale && out, "null buffer");
+    need(aligned16(a) && ld_a % 16 == 0 && aligned16(w) && ld_w % 16 == 0,
+         "rows of a and w must start on 16-byte boundaries");
+    F8Shape s{};
+    s.M = static_cast<int>(M), s.N = static_cast<int>(N), s.K = static_cast<int>(K);
+    s.sa = a_scale, s.sw = w_scale;
+    s.ld_sa = ld_a_scale, s.ld_sw = ld_w_scale;
+    s.bias = bias;
+    s.out = out;
+    s.ld_out = ld_out;
+    s.out_aligned = rows16(out, ld_out, out_dtype);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    by_type(out_dtype, [&](auto tag) {
+      using O = decltype(tag);
+      if (M <= 32) launch_f8<true, 32, O>(a, ld_a, w, ld_w, s, status, st);
+      else if (M <= 64) launch_f8<true, 64, O>(a, ld_a, w, ld_w, s, status, st);
+      else launch_f8<false, 128, O>(a, ld_a, w, ld_w, s, status, st);
+    });
+  });
+}
+
+extern "C" VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, const void* h, int64_t ld_h, int h_dtype,
+                                     const float* post_gain, const void* gate, int gate_dtype, int64_t gate_row_stride,
+                                     int64_t gate_col_stride, float residual_scale, float block_scale,
+                                     const float* pre_gain, float eps, int plus_one, int64_t rows, int64_t cols,
+                                     void* h_out, int64_t ld_h_out, void* z, int64_t ld_z, int z_dtype, float* z_scale,
+                                     int64_t ld_z_scale, void* stream, char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(rows >= 0 && rows <= kMaxInt && cols >= 1 && cols <= VDK_NORM_MAX_COLS,
+         "need 0 <= rows < 2^31 and 1 <= cols <= VDK_NORM_MAX_COLS");
+    need(y_dtype >= VDK_FP16 && y_dtype <= VDK_FP32, "y_dtype must be VDK_FP16, VDK_BF16 or VDK_FP32");
+    need(h_dtype == VDK_FP32 || h_dtype == y_dtype, "h_dtype must be VDK_FP32 or y's type");
+    need(!gate || gate_dtype == VDK_FP32 || gate_dtype == y_dtype, "gate_dtype must be VDK_FP32 or y's type");
+    need(!gate || ((gate_col_stride == 0 || gate_col_stride == 1) && gate_row_stride >= 0),
+         "gate strides: 0 or 1 between columns, not negative between rows");
+    need(y || (!post_gain && !gate), "post_gain and gate need y");
+    need(std::isfinite(residual_scale) && std::isfinite(block_scale) && eps >= 0.0f && std::isfinite(eps),
+         "scales must be finite and eps finite and not negative");
+    need(!z == !pre_gain, "z and pre_gain come together");
+    need(!z || (z_dtype >= VDK_FP16 && z_dtype <= VDK_FP8), "z_dtype must be VDK_FP16, VDK_BF16, VDK_FP32 or VDK_FP8");
+    const int64_t kb = (cols + 127) / 128;
+    need((!y || ld_y >= cols) && (!h || ld_h >= cols) && (!h_out || ld_h_out >= cols) && (!z || ld_z >= cols),
+         "a row stride is smaller than its row");
+    if (rows == 0) return;
+    need(y || h, "need a block output or a residual");
+    need(h_out || z, "nothing to write");
+    need(!z || z_dtype != VDK_FP8 || (z_scale && ld_z_scale >= kb), "8-bit z needs z_scale with a row per token");
+    BlockNormParams p{};
+    p.y = y, p.h = h, p.post = post_gain, p.gate = gate;
+    p.gate_f32 = gate_dtype == VDK_FP32;
+    p.gate_row = gate_row_stride, p.gate_col = gate_col_stride;
+    p.pre = pre_gain, p.h_out = h_out, p.z = z, p.z_scale = z_scale;
+    p.ld_y = ld_y, p.ld_h = ld_h, p.ld_h_out = ld_h_out, p.ld_z = ld_z, p.ld_scale = ld_z_scale;
+    p.cols = static_cast<int>(cols);
+    p.out = !z ? kNormOutNone
+               : z_dtype == VDK_FP16 ? kNormOutF16
+               : z_dtype == VDK_BF16 ? kNormOutBF16
+               : z_dtype == VDK_FP32 ? kNormOutF32
+                                     : kNormOutF8;
+    p.residual_scale = residual_scale, p.block_scale = block_scale, p.eps = eps;
+    p.gain_add = plus_one ? 1.0f : 0.0f;
+    p.z_aligned = z && (z_dtype == VDK_FP8 ? (reinterpret_cast<uintptr_t>(z) & 7) == 0 && ld_z % 8 == 0
+                                           : rows16(z, ld_z, z_dtype));
+    const bool al = (!y || rows16(y, ld_y, y_dtype)) && (!h || rows16(h, ld_h, h_dtype)) &&
+                    (!h_out || rows16(h_out, ld_h_out, h_dtype)) && aligned16(post_gain) && aligned16(pre_gain) &&
+                    (!gate || gate_col_stride == 0 || rows16(gate, gate_row_stride, gate_dtype));
+    const int chunks = static_cast<int>((cols + 7) / 8);
+    const int nv = chunks <= 256 ? 1 : chunks <= 512 ? 2 : 4;
+    const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+    const unsigned grid = static_cast<unsigned>(rows);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    by_type(y_dtype, [&](auto ty) {
+      using TY = decltype(ty);
+      auto run = [&](auto th) {
+        using TH = decltype(th);
+        auto go = [&](auto k) { k<<<grid, threads, 0, s>>>(p); };
+        if (!al) {
+          if (nv == 1) go(block_norm_kernel<TY, TH, 1, false>);
+          else if (nv == 2) go(block_norm_kernel<TY, TH, 2, false>);
+          else go(block_norm_kernel<TY, TH, 4, false>);
+        } else {
+          if (nv == 1) go(block_norm_kernel<TY, TH, 1, true>);
+          else if (nv == 2) go(block_norm_kernel<TY, TH, 2, true>);
+          else go(block_norm_kernel<TY, TH, 4, true>);
+        }
+      };
+      if (h_dtype == VDK_FP32) run(float());
+      else run(TY());
+    });
+    launched();
+  });
+}
+
+extern "C" VD_API int vdk_rotary_turns(double theta, int rotary_dim, int scaling, const double* args,
+                                       const double* divisors, uint64_t* turns, float* factor, char* err,
+                                       size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= VDK_ROTARY_MAX_DIM,
+         "rotary_dim must be even, from 2 to VDK_ROTARY_MAX_DIM");
+    need(std::isfinite(theta) && theta > 0.0, "theta must be positive");
+    need(scaling >= VDK_ROPE_NONE && scaling <= VDK_ROPE_DIVISORS, "unknown scaling");
+    need(turns && factor, "null buffer");
+    need(scaling == VDK_ROPE_NONE || args, "the scaling needs its arguments");
+    need(scaling != VDK_ROPE_DIVISORS || divisors, "the scaling needs one divisor per pair");
+    const double pi = 3.141592653589793238462643383279502884;
+    const int half = rotary_dim / 2;
+    const double d = rotary_dim;
+    double m = 1.0, base = theta;
+    const double f = scaling != VDK_ROPE_NONE ? args[0] : 1.0;
+    if (scaling != VDK_ROPE_NONE && scaling != VDK_ROPE_DIVISORS)
+      need(std::isfinite(f) && f >= 1.0, "the scaling factor must be at least 1");
+    double lo = 0.0, hi = 0.0;
+    if (scaling == VDK_ROPE_NTK) {
+      need(rotary_dim > 2, "this scaling needs rotary_dim > 2");
+      base = theta * std::pow(f, d / (d - 2.0));
+    } else if (scaling == VDK_ROPE_YARN) {
+      const double orig = args[1], fast = args[2], slow = args[3];
+      need(orig > 0.0 && fast > slow && slow > 0.0, "need original_max_position > 0 and beta_fast > beta_slow > 0");
+      need(theta != 1.0, "this scaling needs theta != 1");
+      auto dim = [&](double turns_over) {
+        return d * std::log(orig / (turns_over * 2.0 * pi)) / (2.0 * std::log(theta));
+      };
+      lo = std::max(std::floor(dim(fast)), 0.0);
+      hi = std::min(std::ceil(dim(slow)), d - 1.0);
+      m = args[4] > 0.0 ? args[4] : 0.1 * std::log(f) + 1.0;
+    } else if (scaling == VDK_ROPE_LLAMA3) {
+      need(args[1] > 0.0 && args[3] > args[2], "need original_max_position > 0 and high_freq_factor > low_freq_factor");
+    } else if (scaling == VDK_ROPE_DIVISORS) {
+      m = args[0];
+      need(std::isfinite(m) && m > 0.0, "the factor on the rotated values must be positive");
+    }
+    for (int i = 0; i < half; ++i) {
+      double r = std::pow(base, -2.0 * i / d);  // radians per position
+      if (scaling == VDK_ROPE_LINEAR) {
+        r /= f;
+      } else if (scaling == VDK_ROPE_YARN) {
+        const double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+        r = r / f * ramp + r * (1.0 - ramp);
+      } else if (scaling == VDK_ROPE_LLAMA3) {
+        const double t = std::min(std::max((args[1] * r / (2.0 * pi) - args[2]) / (args[3] - args[2]), 0.0), 1.0);
+        r = (1.0 - t) * r / f + t * r;
+      } else if (scaling == VDK_ROPE_DIVISORS) {
+        need(std::isfinite(divisors[i]) && divisors[i] > 0.0, "divisors must be positive");
+        r /= divisors[i];
+      }
+      const double t = r / (2.0 * pi);
+      const double frac = t - std::floor(t);
+      // frac < 1, and a double has 53 bits: the product is exact, below 2^64.
+      turns[i] = static_cast<uint64_t>(std::ldexp(frac, 64));
+    }
+    *factor = static_cast<float>(m);
+  });
+}
+
+extern "C" VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_heads* k, int64_t tokens, int head_dim,
+                                 int rotary_dim, int dtype, int interleaved, int inverse, const void* positions,
+                                 int positions_bits, int64_t first_position, const uint64_t* turns, float factor,
+                                 void* stream, char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(tokens >= 0 && tokens <= (int64_t(1) << 32), "need 0 <= tokens <= 2^32");
+    need(head_dim >= 2 && head_dim <= 65536 && rotary_dim >= 2 && rotary_dim <= head_dim && rotary_dim % 2 == 0 &&
+             rotary_dim <= VDK_ROTARY_MAX_DIM,
+         "rotary_dim must be even, from 2 to head_dim and to VDK_ROTARY_MAX_DIM");
+    need(!positions || positions_bits == 32 || positions_bits == 64, "positions are 32- or 64-bit");
+    need(q || k, "need queries or keys");
+    need(std::isfinite(factor), "factor must be finite");
+    RotaryParams p{};
+    const int es = elem_bytes(dtype);
+    bool vec = rotary_dim % 8 == 0 && (head_dim - rotary_dim) % 8 == 0 && (interleaved || rotary_dim % 16 == 0);
+    int64_t heads = 0;
+    auto fill = [&](const vdk_rotary_heads* v, RotaryHeads& r) {
+      if (!v) return;
+      need(v->heads >= 1 && v->heads <= 65536, "heads must be from 1 to 65536");
+      need(tokens == 0 || (v->in && v->out), "null buffer");
+      need(v->in_token >= 0 && v->in_head >= 0 && v->out_token >= 0 && v->out_head >= 0, "negative stride");
+      need(v->heads == 1 || v->out_head >= head_dim, "output heads overlap");
+      r = {v->in, v->out, v->in_token, v->in_head, v->out_token, v->out_head, v->heads};
+      for (const int64_t st : {v->in_token, v->in_head, v->out_token, v->out_head}) vec = vec && st * es % 16 == 0;
+      vec = vec && aligned16(v->in) && aligned16(v->out);
+      heads += v->heads;
+    };
+    fill(q, p.q);
+    fill(k, p.k);
+    need(heads * head_dim <= (int64_t(1) << 28), "too many heads");
+    if (tokens == 0) return;
+    need(turns != nullptr, "null buffer");
+    p.positions = positions;
+    p.positions64 = positions_bits == 64;
+    p.first_position = first_position;
+    p.tokens = tokens;
+    p.turns = turns;
+    p.head_dim = head_dim, p.rotary_dim = rotary_dim, p.interleaved = interleaved != 0;
+    p.factor = factor;
+    p.sin_sign = inverse ? -1.0f : 1.0f;
+    const unsigned grid = static_cast<unsigned>((tokens + kRotaryTokens - 1) / kRotaryTokens);
+    const size_t smem = kRotaryTokens * (rotary_dim / 2) * sizeof(float2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    by_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      if (vec) rotary_kernel<T, true><<<grid, kRotaryThreads, smem, s>>>(p);
+      else rotary_kernel<T, false><<<grid, kRotaryThreads, smem, s>>>(p);
+    });
+    launched();
+  });
+}
+
+extern "C" VD_API int vdk_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int dtype,
+                                         float temperature, const int64_t* targets, int64_t n_targets, int top,
+                                         float* logprobs, float* entropy, float* lse, int32_t* top_ids,
+                                         float* top_logprobs, void* stream, char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need(rows >= 0 && rows <= kMaxInt / 8 && vocab >= 1 && vocab <= kMaxInt - 65536,
+         "need 0 <= rows < 2^28 and 1 <= vocab < 2^31 - 65536");
+    need(ld >= vocab, "a row stride is smaller than its row");
+    need(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(1.0f / temperature),
+         "temperature must be positive");
+    need(top >= 0 && top <= VDK_LOGPROBS_MAX_TOP, "top must be from 0 to VDK_LOGPROBS_MAX_TOP");
+    need(n_targets >= 0 && n_targets <= kMaxInt, "n_targets must not be negative");
+    if (rows == 0) return;
+    need(logits != nullptr, "null buffer");
+    need(n_targets == 0 || (targets && logprobs), "targets need their ids and an output");
+    need(top == 0 || (top_ids && top_logprobs), "alternatives need their outputs");
+    need(reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype) == 0, "logits are not aligned to their type");
+    static_assert(VDK_LOGPROBS_MAX_TOP == kLpMaxTop, "");
+    LogprobParams p{};
+    p.logits = logits;
+    p.ld = ld, p.rows = rows;
+    p.vocab = static_cast<int>(vocab);
+    p.targets = targets;
+    p.n_targets = static_cast<int>(n_targets);
+    p.top = top;
+    p.inv_temperature = 1.0f / temperature;
+    p.logprobs = logprobs, p.entropy = entropy, p.lse = lse, p.top_ids = top_ids, p.top_logprobs = top_logprobs;
+    // CTAs share a row while that leaves at most two per SM and each keeps a
+    // batch of loads (kLpThreads * kLpUnroll * 16 bytes) or so.
+    p.splits = 1;
+    const int64_t bytes = vocab * elem_bytes(dtype);
+    while (p.splits < kLpMaxSplits && rows * p.splits * 2 <= 2 * sm_count() && bytes / (p.splits * 2) >= 16384)
+      p.splits *= 2;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    by_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      launch_cluster(token_logprobs_kernel<T>, dim3(static_cast<unsigned>(rows * p.splits)), kLpThreads,
+                     sizeof(LpShared), p.splits, s, p);
+    });
+  });
+}

@@ -1,0 +1,119 @@
+// Casts to 8-bit floating point (e4m3) with an fp32 scale per block.
+//
+// Activations: for each row and block of 128 columns, with v = x or
+// v = act(gate) * x,
+//   a = max(max |v|, 1e-30),  scale = a / 448,  q = e4m3(v * (448 / a)).
+// A block that holds inf or NaN gets that as its scale, so that the whole
+// block stands for non-finite values and the product's row shows it.
+//
+// Bound by memory: one read of x (and gate), one write of a byte per element.
+// 16 lanes hold a block (8 elements each, one 16-byte load for 16-bit types),
+// so its maximum is four shuffles; each thread takes kQuantUnroll blocks,
+// whose loads are all issued before the first is used.
+#pragma once
+
+#include "gemm.cuh"
+#include "row_io.cuh"
+
+namespace vd {
+
+struct QuantizeParams {
+  const void* x;
+  const void* gate;
+  int64_t ld_x, ld_gate, ld_q, ld_scale;
+  uint32_t blocks, col_blocks;  // rows * col_blocks, ceil(cols / 128)
+  int cols, act;
+  uint8_t* q;
+  float* scale;
+  bool q_aligned;
+};
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantUnroll = 4;
+
+__device__ __forceinline__ float gate_act(float g, int act) {
+  if (act == kActSilu) return __fdividef(g, 1.0f + __expf(-g));
+  return apply_act(g, act);
+}
+
+template <class T, bool GATED, bool ALIGNED>
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantizeParams p) {
+  const int lane16 = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (kQuantUnroll * kQuantThreads / 16) + (threadIdx.x >> 4);
+  Chunk8<T> xr[kQuantUnroll], gr[kQuantUnroll];
+#pragma unroll
+  for (int u = 0; u < kQuantUnroll; ++u) {
+    const uint32_t id = first + u * (kQuantThreads / 16);
+    const uint32_t row = id / p.col_blocks;
+    const int col = static_cast<int>(id - row * p.col_blocks) * kF8Block + lane16 * 8;
+    const int n = id < p.blocks ? p.cols - col : 0;
+    const T* x = static_cast<const T*>(p.x) + row * p.ld_x + col;
+    const T* g = GATED ? static_cast<const T*>(p.gate) + row * p.ld_gate + col : nullptr;
+    if (ALIGNED && n >= 8) {
+      xr[u].load(x);
+      if (GATED) gr[u].load(g);
+    } else {
+      xr[u].load_part(x, n);
+      if (GATED) gr[u].load_part(g, n);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantUnroll; ++u) {
+    const uint32_t id = first + u * (kQuantThreads / 16);
+    const uint32_t row = id / p.col_blocks;
+    const uint32_t kb = id - row * p.col_blocks;
+    const int col = static_cast<int>(kb) * kF8Block + lane16 * 8;
+    float v[8];
+    xr[u].get(v);
+    if (GATED) {
+      float g[8];
+      gr[u].get(g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= gate_act(g[j], p.act);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, magnitude_bits(v[j]));
+    const F8Scale s = f8_scale(max16(m));
+    if (id < p.blocks) {
+      if (lane16 == 0) p.scale[row * p.ld_scale + kb] = s.scale;
+      f8_store(p.q + row * p.ld_q + col, f8_pack8(v, s.inv), p.cols - col, p.q_aligned);
+    }
+  }
+}
+
+// Weights, once at load: a block is 128 rows x 128 columns, one CTA each.
+template <class T>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const T* __restrict__ w, int64_t ld_w, int rows, int cols,
+                                                              uint8_t* __restrict__ q, int64_t ld_q,
+                                                              float* __restrict__ scale, int64_t ld_scale) {
+  __shared__ uint32_t warp_max[8];
+  const int col = blockIdx.x * kF8Block + (threadIdx.x & 15) * 8;
+  const int row0 = blockIdx.y * kF8Block + (threadIdx.x >> 4);
+  float v[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = row0 + i * 16;
+    Chunk8<T> c;
+    c.zero();
+    if (row < rows && col < cols) c.load_part(w + row * ld_w + col, cols - col);
+    c.get(v[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, magnitude_bits(v[i][j]));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, warp_max[i]);
+  const F8Scale s = f8_scale(m);
+  if (threadIdx.x == 0) scale[blockIdx.y * ld_scale + blockIdx.x] = s.scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = row0 + i * 16;
+    if (row < rows && col < cols) f8_store(q + row * ld_q + col, f8_pack8(v[i], s.inv), cols - col, false);
+  }
+}
+
+}  // namespace vd

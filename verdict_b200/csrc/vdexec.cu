@@ -44,19 +44,13 @@
 #include "gemm.cuh"
 #include "gemm2.cuh"
 #include "gdn.cuh"
+#include "host.hpp"
 #include "json.hpp"
 #include "synth.cuh"
 
 namespace vd {
 
 using bf16 = __nv_bfloat16;
-
-struct VdError {
-  int code;
-  std::string msg;
-};
-
-[[noreturn]] static void fail(int code, const std::string& msg) { throw VdError{code, msg}; }
 
 // Fused RMSNorm with fp16 activations: the 16-bit copy of the residual rows
 // (times the norm's gains) is stored times 2^-6, so rows up to 4.2e6 in
@@ -86,10 +80,6 @@ static int choose_splits(int tiles, int kblocks, int sms, int max_splits) {
     }
   }
   return pick;
-}
-
-static void cuda_check(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) fail(VD_ECUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 // ---------------------------------------------------------------------------
@@ -538,24 +528,6 @@ static uint64_t tensor_base(uint64_t seed, const std::string& name) {
 // ---------------------------------------------------------------------------
 // Tensor maps
 // ---------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  if (!fn) fail(VD_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  return fn;
-}
-
 // Row-major [rows, cols] 16-bit matrix, box = [box_rows, 64] with 128-byte swizzle.
 static CUtensorMap make_map(const void* ptr, int64_t rows, int64_t cols, int box_rows, bool f16 = true) {
   CUtensorMap m;
@@ -2366,13 +2338,6 @@ static void check_device_error(vd_handle* H) {
 // C ABI
 // ---------------------------------------------------------------------------
 using namespace vd;
-
-static void put_err(char* err, size_t errlen, const std::string& msg) {
-  if (!err || errlen == 0) return;
-  const size_t n = std::min(errlen - 1, msg.size());
-  std::memcpy(err, msg.data(), n);
-  err[n] = '\0';
-}
 
 template <class F>
 static int guarded(vd_handle* h, char* err, size_t errlen, F&& body) {
