@@ -9,13 +9,8 @@
 // times its scale, to fp32 sums that stay in registers over the whole of K.
 // Several TMEM accumulators keep the MMAs ahead of the drain.
 //
-// One-CTA kernel (this file's first): a tile is 128 rows of P by BN rows of Q.
-//   SWAP = false: P = a (a thread of the drain owns a token; its scale is one
-//     number per k-block), Q = w.
-//   SWAP = true: P = w, Q = a, for few tokens: the 128-row side of the MMA is
-//     filled with weight rows, and a tile needs no more than 32 or 64 tokens.
-// Where the tiles do not fill the GPU, a cluster of CTAs splits K and joins its
-// sums through distributed shared memory, in rank order.
+// Two kernels: fp8_gemm_pair_kernel (CTA pairs, 256 x 256 tiles) for many
+// rows, fp8_gemm_rows_kernel (below) for few.
 #pragma once
 
 #include "gemm2.cuh"
@@ -35,6 +30,28 @@ struct F8Shape {
   int splits;       // CTAs along K: the cluster's size
 };
 
+// mbar_wait with the clock read only after a run of polls: reading the global
+// timer takes longer than the k-block that most waits here are for.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+      if (*abort_flag) return false;
+    }
+    const uint64_t t = globaltimer();
+    if (t0 == 0) {
+      t0 = t;
+    } else if (t - t0 > VD_WAIT_TIMEOUT_NS) {
+      *abort_flag = 1;
+      record_error(err, code);
+      return false;
+    }
+  }
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, e4m3 inputs, fp32 accumulate.
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -49,50 +66,113 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
 // e4m3 x e4m3 -> fp32, both operands K-major: the format codes are 0.
 __host__ __device__ constexpr uint32_t umma_idesc_f8(int m, int n) { return umma_idesc_f16kind(m, n, 0); }
 
-template <int BN>
-struct F8Config {
-  static constexpr int BM = 128;
-  static constexpr int BK = 128;
-  static constexpr int STAGES = BN == 128 ? 6 : 8;
-  static constexpr int P_BYTES = BM * BK;
-  static constexpr int Q_BYTES = BN * BK;
-  static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-  static constexpr int BUFS = 4;  // TMEM accumulators
-  static constexpr int TMEM_COLS = BUFS * BN;
-  static constexpr int SCALE_KB = 16;  // k-blocks of token scales staged at a time (SWAP)
-  static constexpr int SCALE_BYTES = 2 * SCALE_KB * BN * 4;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 1024 + SCALE_BYTES;
-  static constexpr int THREADS = 192;
-};
-
-__device__ __forceinline__ void drain_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-
-template <class O>
-__device__ __forceinline__ void f8_out(O* out, float v, int n, const float* bias) {
-  *out = Elem<O>::from(bias ? v + __ldg(bias + n) : v);
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
 }
 
-template <bool SWAP, int BN, class O>
-__global__ void __launch_bounds__(F8Config<BN>::THREADS, 1)
-    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, F8Shape s,
-                    int* err) {
-  using Cfg = F8Config<BN>;
-  constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS;
-  constexpr uint32_t IDESC = umma_idesc_f8(Cfg::BM, BN);
+// N = 16, 32 or 64 consecutive columns of this thread's TMEM lane.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
+  static_assert(N == 16 || N == 32 || N == 64, "");
+  if constexpr (N == 32) {
+    tmem_ld32(taddr, r);
+  } else if constexpr (N == 16) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the weights are read once and everything else is small, so this
+// side is bound by memory and, for the shortest calls, by latency.
+//
+// A tile is 128 weight rows (the 128-row side of the MMA) by BN tokens; a CTA
+// owns one tile over its share of K.  Where the tiles do not fill the GPU, a
+// cluster of CTAs splits K: each CTA pushes its sums to the CTA that owns a
+// token's column through distributed shared memory, and that one adds them in
+// rank order, so the result does not depend on who came first.
+//
+// A drain thread owns a weight row.  The scales a[token] * w of 16 k-blocks at
+// a time lie in shared memory and are read four tokens at once.
+// ---------------------------------------------------------------------------
+template <int BN>
+struct F8RowsConfig {
+  static constexpr int BM = 128;
+  static constexpr int BK = 128;
+  static constexpr int STAGES = BN == 128 ? 4 : BN == 64 ? 6 : 8;
+  static constexpr int W_BYTES = BM * BK;
+  static constexpr int A_BYTES = BN * BK;
+  static constexpr int STAGE_BYTES = W_BYTES + A_BYTES;
+  static constexpr int BUFS = 4;  // TMEM accumulators
+  static constexpr int TMEM_COLS = BUFS * BN;
+  static constexpr int DRAIN_WARPS = BN >= 64 ? 8 : 4;
+  static constexpr int COLS = BN / (DRAIN_WARPS / 4);  // columns of a drain warp
+  static constexpr int SCALE_KB = 16;
+  static constexpr int SCALE_BYTES = 2 * SCALE_KB * BN * 4;
+  static constexpr int MAX_SPLITS = 8;
+  static constexpr int SUM_BYTES = (BN + MAX_SPLITS) * BM * 4;  // what the cluster's CTAs send here
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + SCALE_BYTES + SUM_BYTES + 512;
+  static constexpr int THREADS = 64 + 32 * DRAIN_WARPS;
+};
+
+template <int BN, class O>
+__global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
+    fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, F8Shape s,
+                         int* err) {
+  using Cfg = F8RowsConfig<BN>;
+  constexpr int BM = Cfg::BM, BK = Cfg::BK, STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, COLS = Cfg::COLS;
+  constexpr int DRAIN = 32 * Cfg::DRAIN_WARPS;
+  constexpr uint32_t IDESC = umma_idesc_f8(BM, BN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sP = smem;
-  uint8_t* sQ = smem + STAGES * Cfg::P_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+  uint8_t* sW = smem;
+  uint8_t* sA = smem + STAGES * Cfg::W_BYTES;
+  float* sScale = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);
+  float* sSum = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALE_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALE_BYTES + Cfg::SUM_BYTES);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + BUFS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sScale = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES + 1024);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
+  const int kblocks = (s.K + BK - 1) / BK;
+  const int tile = static_cast<int>(blockIdx.x) / s.splits;
+  const int part = static_cast<int>(blockIdx.x) - tile * s.splits;
+  const int n0 = tile * BM;
+  const int m0 = static_cast<int>(blockIdx.y) * BN;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(kblocks) * part / s.splits);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(kblocks) * (part + 1) / s.splits);
+
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
@@ -100,7 +180,7 @@ __global__ void __launch_bounds__(F8Config<BN>::THREADS, 1)
     }
     for (int i = 0; i < BUFS; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4);
+      mbar_init(&acc_empty[i], Cfg::DRAIN_WARPS);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -111,163 +191,157 @@ __global__ void __launch_bounds__(F8Config<BN>::THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // Says that this CTA runs: its shared memory may be written once all have.
+  if (s.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int kblocks = (s.K + Cfg::BK - 1) / Cfg::BK;
-  const int part = static_cast<int>(blockIdx.x) % s.splits;
-  const int p0 = static_cast<int>(blockIdx.x) / s.splits * Cfg::BM;
-  const int q0 = static_cast<int>(blockIdx.y) * BN;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(kblocks) * part / s.splits);
-  const int kb1 = static_cast<int>(static_cast<int64_t>(kblocks) * (part + 1) / s.splits);
-
-  float acc[BN];
+  float acc[COLS];
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_desc(&tmP);
-      tma_prefetch_desc(&tmQ);
       int stage = 0;
       uint32_t phase = 0;
+      bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty)) break;
+        ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
+        if (!ok) break;
         mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
-        tma_load_2d(sP + stage * Cfg::P_BYTES, &tmP, &full[stage], kb * Cfg::BK, p0);
-        tma_load_2d(sQ + stage * Cfg::Q_BYTES, &tmQ, &full[stage], kb * Cfg::BK, q0);
+        tma_load_2d(sW + stage * Cfg::W_BYTES, &tmW, &full[stage], kb * BK, n0);
+        tma_load_2d(sA + stage * Cfg::A_BYTES, &tmA, &full[stage], kb * BK, m0);
         if (++stage == STAGES) stage = 0, phase ^= 1;
       }
       // Every load has landed and been consumed before the CTA may exit.
-      for (int i = 0; i < STAGES; ++i) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty)) break;
+      for (int i = 0; i < STAGES && ok; ++i) {
+        ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
         if (++stage == STAGES) stage = 0, phase ^= 1;
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty)) break;
-        if (!mbar_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull)) break;
-        tc_fence_after();
-        const uint32_t p_addr = smem_u32(sP + stage * Cfg::P_BYTES);
-        const uint32_t q_addr = smem_u32(sQ + stage * Cfg::Q_BYTES);
+    int stage = 0, buf = 0;
+    uint32_t phase = 0, buf_phase = 0;
+    const uint64_t w_desc0 = sw128_kmajor_desc(smem_u32(sW)), a_desc0 = sw128_kmajor_desc(smem_u32(sA));
+    for (int kb = kb0; kb < kb1; ++kb) {
+      bool ok = f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty) &&
+                f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        // Descriptors hold addresses in units of 16 bytes; 32 bytes per step of K.
+        const uint64_t w_desc = w_desc0 + stage * (Cfg::W_BYTES >> 4);
+        const uint64_t a_desc = a_desc0 + stage * (Cfg::A_BYTES >> 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_f8(tmem_base + buf * BN, sw128_kmajor_desc(p_addr + k * 32), sw128_kmajor_desc(q_addr + k * 32), IDESC,
-                  k != 0);
-        umma_commit(&empty[stage]);
+          umma_f8(tmem_base + buf * BN, w_desc + 2 * k, a_desc + 2 * k, IDESC, k != 0);
         umma_commit(&acc_full[buf]);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
-        if (++buf == BUFS) buf = 0, buf_phase ^= 1;
+        umma_commit(&empty[stage]);
       }
+      __syncwarp();
+      if (++stage == STAGES) stage = 0, phase ^= 1;
+      if (++buf == BUFS) buf = 0, buf_phase ^= 1;
     }
   } else {
-    // Drain: thread (lane quarter warp % 4, lane) owns row p of the tile.
+    // Drain: TMEM lane quarter warp % 4, columns [COLS * part, ...).
     const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
+    const int col0 = ((warp - 2) >> 2) * COLS;
     const int t = threadIdx.x - 64;
-    const int p = p0 + row;
-    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
+    const float* sw = s.sw + static_cast<int64_t>(n0 / kF8Block) * s.ld_sw;
+    constexpr int PER = Cfg::SCALE_KB * BN / DRAIN;  // scales of a chunk per thread
+    float next[PER];
+    auto fetch = [&](int base) {
 #pragma unroll
-    for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
-    int buf = 0;
-    uint32_t buf_phase = 0;
-    // SWAP: one weight-block scale for the whole tile, a scale per column
-    // (token), staged SCALE_KB k-blocks at a time.  Otherwise: one scale per
-    // thread (token) and one for the tile (BN = 128: one weight block).
-    const float* sw = s.sw + static_cast<int64_t>((SWAP ? p0 : q0) / kF8Block) * s.ld_sw;
-    const float* sa = !SWAP && p < s.M ? s.sa + p * s.ld_sa : nullptr;
-    bool ok = true;
-    for (int base = kb0; base < kb1 && ok; base += Cfg::SCALE_KB) {
-      const int stop = min(base + Cfg::SCALE_KB, kb1);
-      float* scales = sScale + ((base - kb0) / Cfg::SCALE_KB & 1) * (Cfg::SCALE_KB * BN);
-      if constexpr (SWAP) {
-        // Column-major by k-block; two buffers: the barrier below also tells
-        // that every warp is done with the buffer before last.
-        for (int i = t; i < Cfg::SCALE_KB * BN; i += 128) {
-          const int tok = i / Cfg::SCALE_KB, kb = base + i % Cfg::SCALE_KB;
-          scales[i % Cfg::SCALE_KB * BN + tok] =
-              q0 + tok < s.M && kb < stop ? __ldg(s.sa + (q0 + tok) * s.ld_sa + kb) : 0.0f;
-        }
-        drain_barrier();
+      for (int i = 0; i < PER; ++i) {
+        const int e = i * DRAIN + t;
+        const int tok = m0 + e / Cfg::SCALE_KB, kb = base + e % Cfg::SCALE_KB;
+        next[i] = tok < s.M && kb < kb1 ? __ldg(s.sa + tok * s.ld_sa + kb) * __ldg(sw + kb) : 0.0f;
       }
-      for (int kb = base; kb < stop; ++kb) {
-        const float w = __ldg(sw + kb);
-        const float f = SWAP ? w : w * (sa ? __ldg(sa + kb) : 0.0f);
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull));
+    };
+    auto put = [&](int chunk) {
+      float* to = sScale + (chunk & 1) * (Cfg::SCALE_KB * BN);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = i * DRAIN + t;
+        to[e % Cfg::SCALE_KB * BN + e / Cfg::SCALE_KB] = next[i];
+      }
+    };
+    fetch(kb0);
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) acc[j] = 0.0f;
+    put(0);
+    int buf = 0, chunk = 0;
+    uint32_t buf_phase = 0;
+    bool ok = true;
+    for (int base = kb0; base < kb1 && ok; base += Cfg::SCALE_KB, ++chunk) {
+      // The chunk is in place; the other buffer's chunk has been used up.
+      asm volatile("bar.sync 1, %0;" ::"n"(DRAIN) : "memory");
+      const int stop = min(base + Cfg::SCALE_KB, kb1);
+      if (stop < kb1) fetch(stop);
+      const float* scales = sScale + (chunk & 1) * (Cfg::SCALE_KB * BN) + col0;
+      for (int kb = base; kb < stop; ++kb, scales += BN) {
+        ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull));
         if (!ok) break;
         tc_fence_after();
-        uint32_t r[2][32];
-        tmem_ld32(taddr + buf * BN, r[0]);
+        uint32_t r[COLS];
+        tmem_ld<COLS>(taddr + buf * BN, r);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          tmem_wait_ld();
-          if (c + 1 < BN / 32) {
-            tmem_ld32(taddr + buf * BN + (c + 1) * 32, r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float d = __uint_as_float(r[c & 1][j]);
-            const float g = SWAP ? f * scales[(kb - base) * BN + c * 32 + j] : f;
-            acc[c * 32 + j] = fmaf(d, g, acc[c * 32 + j]);
-          }
+        for (int j = 0; j < COLS; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(scales + j);
+          acc[j] = fmaf(__uint_as_float(r[j]), f.x, acc[j]);
+          acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), f.y, acc[j + 1]);
+          acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), f.z, acc[j + 2]);
+          acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), f.w, acc[j + 3]);
         }
         if (++buf == BUFS) buf = 0, buf_phase ^= 1;
       }
-    }
-    if (s.splits > 1) {
-      // All MMAs of this CTA are done (its last accumulator was read), so the
-      // stages are free: [column][row], one 128-byte line per warp access.
-      float* sums = reinterpret_cast<float*>(smem);
-#pragma unroll
-      for (int j = 0; j < BN; ++j) sums[j * Cfg::BM + row] = acc[j];
+      if (stop < kb1) put(chunk + 1);
     }
   }
-  if (s.splits > 1) {
-    __syncthreads();
-    cluster_sync_all();
+
+  const int row = (warp & 3) * 32 + lane;  // of a drain thread
+  const int n = n0 + row;
+  O* out = static_cast<O*>(s.out);
+  if (s.splits == 1) {
+    if (warp >= 2 && n < s.N) {
+      const int col0 = ((warp - 2) >> 2) * COLS;
+      const float bias = s.bias ? __ldg(s.bias + n) : 0.0f;
+      O* o = out + static_cast<int64_t>(m0 + col0) * s.ld_out + n;
+#pragma unroll
+      for (int j = 0; j < COLS; ++j)
+        if (m0 + col0 + j < s.M) o[j * s.ld_out] = Elem<O>::from(acc[j] + bias);
+    }
+  } else {
+    // Column j goes to CTA j / share, into [rank][j % share][row].
+    const int share = (BN + s.splits - 1) / s.splits;
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA runs
     if (warp >= 2) {
-      const int quarter = warp & 3;
-      const int row = quarter * 32 + lane;
-      const int p = p0 + row;
-      const int j0 = BN * part / s.splits, j1 = BN * (part + 1) / s.splits;
-      const uint32_t local = smem_u32(smem);
-      O* out = static_cast<O*>(s.out);
-      for (int j = j0; j < j1; ++j) {
-        float v = 0.0f;
-        for (int r = 0; r < s.splits; ++r) {
-          float x;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(x)
-                       : "r"(mapa_shared(local + (j * Cfg::BM + row) * 4, r)));
-          v += x;
-        }
-        const int m = SWAP ? q0 + j : p, n = SWAP ? p : q0 + j;
-        if (m < s.M && n < s.N) f8_out(out + m * s.ld_out + n, v, n, s.bias);
+      const int col0 = ((warp - 2) >> 2) * COLS;
+      const uint32_t mine = smem_u32(sSum) + (part * share * BM + row) * 4;
+      int to = col0 / share, at = col0 - to * share;
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) {
+        if (m0 + col0 + j < s.M)
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(mine + at * (BM * 4), to)), "f"(acc[j])
+                       : "memory");
+        if (++at == share) at = 0, ++to;
       }
     }
-    cluster_sync_all();  // no CTA leaves while its sums are read
-  } else if (warp >= 2) {
-    const int p = p0 + (warp & 3) * 32 + lane;
-    O* out = static_cast<O*>(s.out);
-    if constexpr (SWAP) {
-#pragma unroll
-      for (int j = 0; j < BN; ++j)
-        if (q0 + j < s.M && p < s.N) f8_out(out + (q0 + j) * s.ld_out + p, acc[j], p, s.bias);
-    } else if (p < s.M) {
-      O* o = out + p * s.ld_out + q0;
-#pragma unroll
-      for (int j = 0; j < BN; j += 8) {
-        if (q0 + j >= s.N) break;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = acc[j + i] + (s.bias && q0 + j + i < s.N ? __ldg(s.bias + q0 + j + i) : 0.0f);
-        if (s.out_aligned && q0 + j + 8 <= s.N) store8(o + j, v);
-        else store8_part(o + j, v, s.N - q0 - j);
+    __syncwarp();
+    cluster_sync_all();  // the sums have arrived
+    if (warp >= 2 && n < s.N) {
+      const float bias = s.bias ? __ldg(s.bias + n) : 0.0f;
+      const int first = part * share;
+      const int count = min(min(share, BN - first), s.M - m0 - first);
+      for (int j = (warp - 2) >> 2; j < count; j += Cfg::DRAIN_WARPS / 4) {
+        float v = 0.0f;
+        for (int r = 0; r < s.splits; ++r) v += sSum[(r * share + j) * BM + row];
+        out[static_cast<int64_t>(m0 + first + j) * s.ld_out + n] = Elem<O>::from(v + bias);
       }
     }
   }
@@ -278,6 +352,291 @@ __global__ void __launch_bounds__(F8Config<BN>::THREADS, 1)
   if (warp == 1) {
     __syncwarp();
     tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// CTA pairs (cta_group::2): 256 x 256 tiles for shapes with enough of them.
+//
+// A pair stages 2 x 32 KB per k-block for 256 x 256 x 128 products, a third
+// less shared-memory traffic per product than 128 x 256 tiles on one CTA.  The
+// MMAs of a k-block write one of two 256-column TMEM accumulators; eight drain
+// warps per CTA (two per TMEM lane quarter, 128 columns each) add it to their
+// registers while the next k-block's MMAs fill the other.  The grid is
+// persistent, one pair per two SMs; outputs leave through shared memory and
+// TMA stores while the next tile's MMAs run.
+// ---------------------------------------------------------------------------
+struct F8PairConfig {
+  static constexpr int BM = 128;  // rows per CTA
+  static constexpr int BN = 256;
+  static constexpr int BK = 128;
+  static constexpr int STAGES = 6;
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int B_BYTES = BN / 2 * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int DRAIN_WARPS = 8;
+  static constexpr int OUT_BYTES = 4096;  // per drain warp: 32 rows of 128 bytes
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + DRAIN_WARPS * OUT_BYTES + 1024;
+  static constexpr int THREADS = 128 + 32 * DRAIN_WARPS;
+  // Registers: the launch's 168 a thread are redistributed, 40 to the control
+  // warpgroup and 232 to the two of the drain.
+  static constexpr int LAUNCH_REGS = 168, CONTROL_REGS = 40, DRAIN_REGS = 232;
+  static_assert(128 * CONTROL_REGS + 256 * DRAIN_REGS <= THREADS * LAUNCH_REGS, "register split");
+  static constexpr int GROUP_M = 8;  // pair tiles (256 rows) per raster group
+};
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on an mbarrier of either CTA with the default semantics.  What it
+// tells the leader is that this warp's TMEM loads are complete, which
+// tcgen05.wait::ld and the tcgen05 fences order; no memory access is handed
+// over.  (mbarrier.arrive.release.cluster is a memory barrier on top, which
+// waited for the scale loads in flight: 600 cycles a k-block.)
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+template <class O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREADS, 1)
+    fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         const __grid_constant__ CUtensorMap tmC, F8Shape s, int* err) {
+  using Cfg = F8PairConfig;
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, BK = Cfg::BK, STAGES = Cfg::STAGES;
+  constexpr uint32_t IDESC = umma_idesc_f8(2 * BM, BN);
+  constexpr int CHUNK = 128 / sizeof(O);  // columns of a 128-byte output row in shared memory
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
+  uint8_t* sOut = smem + STAGES * Cfg::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + Cfg::DRAIN_WARPS * Cfg::OUT_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);   // the leader's arm; both CTAs' bytes complete it
+      mbar_init(&empty[i], 1);  // the leader's commit, multicast to both CTAs
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * Cfg::DRAIN_WARPS);  // both CTAs' drain warps (the leader's copy is used)
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrive
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int num_m = (s.M + 2 * BM - 1) / (2 * BM);
+  const int num_n = (s.N + BN - 1) / BN;
+  const int tiles = num_m * num_n;
+  const int kblocks = (s.K + BK - 1) / BK;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::CONTROL_REGS));
+    if (warp == 0) {
+      if (lane == 0) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+        tma_prefetch_desc(&tmC);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+          int m, n;
+          tile_coords(tile, num_m, num_n, Cfg::GROUP_M, m, n);
+          const int ya = m * 2 * BM + static_cast<int>(rank) * BM;
+          const int yb = n * BN + static_cast<int>(rank) * (BN / 2);
+          for (int kb = 0; kb < kblocks; ++kb) {
+            if (!f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty)) {
+              ok = false;
+              break;
+            }
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
+            const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+            tma_load_2d_pair(sA + stage * Cfg::A_BYTES, &tmA, bar, kb * BK, ya);
+            tma_load_2d_pair(sB + stage * Cfg::B_BYTES, &tmB, bar, kb * BK, yb);
+            if (++stage == STAGES) stage = 0, phase ^= 1;
+          }
+        }
+        // Every stage this CTA filled has been consumed before the CTA may exit.
+        for (int i = 0; i < STAGES && ok; ++i) {
+          ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+      }
+    } else if (warp == 1) {
+      // The whole warp waits and one elected lane issues, so that addresses and
+      // descriptors stay in uniform registers: with a k-block's MMAs over in 512
+      // cycles, what the issuing thread does between them counts.
+      if (leader) {
+        int stage = 0, buf = 0;
+        uint32_t phase = 0, buf_phase = 0;
+        const uint64_t a_desc0 = sw128_kmajor_desc(smem_u32(sA)), b_desc0 = sw128_kmajor_desc(smem_u32(sB));
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+          for (int kb = 0; kb < kblocks; ++kb) {
+            ok = f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull) &&
+                 f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              // Descriptors hold addresses in units of 16 bytes; 32 bytes per step of K.
+              const uint64_t a_desc = a_desc0 + stage * (Cfg::A_BYTES >> 4);
+              const uint64_t b_desc = b_desc0 + stage * (Cfg::B_BYTES >> 4);
+              const uint32_t d = tmem_base + buf * BN;
+              umma_f8_pair(d, a_desc, b_desc, IDESC, 0);
+              umma_f8_pair(d, a_desc + 2, b_desc + 2, IDESC, 1);
+              umma_f8_pair(d, a_desc + 4, b_desc + 4, IDESC, 1);
+              umma_f8_pair(d, a_desc + 6, b_desc + 6, IDESC, 1);
+              umma_commit_pair(&acc_full[buf], 0x3);
+              umma_commit_pair(&empty[stage], 0x3);
+            }
+            __syncwarp();
+            if (++stage == STAGES) stage = 0, phase ^= 1;
+            if (++buf == 2) buf = 0, buf_phase ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::DRAIN_REGS));
+    // Drain warp: TMEM lane quarter warp % 4, columns [128 half, +128), one
+    // weight block: thread = output row, one scale per k-block.
+    const int quarter = warp & 3;
+    const int half = (warp - 4) >> 2;
+    uint8_t* stage_out = sOut + (warp - 4) * Cfg::OUT_BYTES;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    const uint32_t release0 = mapa_shared(smem_u32(&acc_empty[0]), 0);
+    const uint32_t release1 = mapa_shared(smem_u32(&acc_empty[1]), 0);
+    const int wblocks = (s.N + kF8Block - 1) / kF8Block;
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs) {
+      int m, n;
+      tile_coords(tile, num_m, num_n, Cfg::GROUP_M, m, n);
+      const int row0 = m * 2 * BM + static_cast<int>(rank) * BM + quarter * 32;
+      const int row = row0 + lane;
+      const int col0 = n * BN + half * 128;
+      // Rows and blocks past the end: any scale, their products are zero.
+      const float* sa = s.sa + min(row, s.M - 1) * s.ld_sa;
+      const float* sw = s.sw + min(col0 / kF8Block, wblocks - 1) * s.ld_sw;
+      float2 acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+      // Scales are loaded two k-blocks ahead.
+      float a1 = __ldg(sa), w1 = __ldg(sw);
+      float a2 = kblocks > 1 ? __ldg(sa + 1) : 0.0f, w2 = kblocks > 1 ? __ldg(sw + 1) : 0.0f;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        const float f = a1 * w1;
+        a1 = a2, w1 = w2;
+        if (kb + 2 < kblocks) a2 = __ldg(sa + kb + 2), w2 = __ldg(sw + kb + 2);
+        ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull));
+        if (!ok) break;
+        tc_fence_after();
+        const float2 ff = make_float2(f, f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[64];
+          tmem_ld<64>(taddr + buf * BN + c * 64, r);
+          tmem_wait_ld();
+          if (c == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_remote(buf ? release1 : release0);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            acc[c * 32 + j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), ff,
+                                         acc[c * 32 + j]);
+        }
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
+      }
+      if (!ok) break;
+      if (s.bias) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          const int col = col0 + 2 * j;
+          if (col < s.N) acc[j].x += __ldg(s.bias + col);
+          if (col + 1 < s.N) acc[j].y += __ldg(s.bias + col + 1);
+        }
+      }
+      if (!s.out_aligned) {  // rows of out that TMA cannot address
+        if (row < s.M) {
+          O* o = static_cast<O*>(s.out) + row * s.ld_out + col0;
+#pragma unroll
+          for (int j = 0; j < 64; ++j) {
+            if (col0 + 2 * j < s.N) o[2 * j] = Elem<O>::from(acc[j].x);
+            if (col0 + 2 * j + 1 < s.N) o[2 * j + 1] = Elem<O>::from(acc[j].y);
+          }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int c = 0; c < 128 / CHUNK; ++c) {
+        const int x = col0 + c * CHUNK;
+        if (x >= s.N || row0 >= s.M) break;
+        if (lane == 0) bulk_wait_read<0>();  // the store before has read the buffer
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          uint4 w;
+          const float2* v = acc + c * (CHUNK / 2) + q * (CHUNK / 16);
+          if constexpr (sizeof(O) == 4) {
+            w = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+                           __float_as_uint(v[1].y));
+          } else {
+            w = make_uint4(Elem<O>::pack2(v[0].x, v[0].y), Elem<O>::pack2(v[1].x, v[1].y),
+                           Elem<O>::pack2(v[2].x, v[2].y), Elem<O>::pack2(v[3].x, v[3].y));
+          }
+          *reinterpret_cast<uint4*>(stage_out + lane * 128 + ((q ^ (lane & 7)) << 4)) = w;
+        }
+        fence_proxy_async_smem_gemm();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmC, stage_out, x, row0);
+          bulk_commit();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while its peer may still read or signal its shared memory
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
   }
 }
 

@@ -89,24 +89,59 @@ CUtensorMap f8_map(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int 
   return m;
 }
 
-template <bool SWAP, int BN, class O>
-void launch_f8(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8Shape s, int* status, cudaStream_t stream) {
-  using Cfg = F8Config<BN>;
-  auto kernel = fp8_gemm_kernel<SWAP, BN, O>;
+template <int BN, class O>
+void launch_f8_rows(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8Shape s, int* status,
+                    cudaStream_t stream) {
+  using Cfg = F8RowsConfig<BN>;
+  auto kernel = fp8_gemm_rows_kernel<BN, O>;
   cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES),
              "shared memory size");
-  const CUtensorMap ma = f8_map(a, s.M, s.K, ld_a, SWAP ? BN : 128);
-  const CUtensorMap mw = f8_map(w, s.N, s.K, ld_w, SWAP ? 128 : BN);
-  const int p_tiles = ((SWAP ? s.N : s.M) + 127) / 128;
-  const int q_tiles = ((SWAP ? s.M : s.N) + BN - 1) / BN;
+  const int n_tiles = (s.N + 127) / 128, m_tiles = (s.M + BN - 1) / BN;
   // K is split while the CTAs still fit on the GPU at once (one per SM) and
   // each keeps at least four k-blocks.
   const int kblocks = (s.K + 127) / 128;
-  const int tiles = p_tiles * q_tiles;
+  const int tiles = n_tiles * m_tiles;
   s.splits = 1;
-  while (s.splits < 8 && tiles * (s.splits + 1) <= sm_count() && kblocks / (s.splits + 1) >= 4) ++s.splits;
-  launch_cluster(kernel, dim3(p_tiles * s.splits, q_tiles), Cfg::THREADS, Cfg::SMEM_BYTES, s.splits, stream,
-                 SWAP ? mw : ma, SWAP ? ma : mw, s, status);
+  while (s.splits < Cfg::MAX_SPLITS && tiles * (s.splits + 1) <= sm_count() && kblocks / (s.splits + 1) >= 4) ++s.splits;
+  launch_cluster(kernel, dim3(n_tiles * s.splits, m_tiles), Cfg::THREADS, Cfg::SMEM_BYTES, s.splits, stream,
+                 f8_map(w, s.N, s.K, ld_w, 128), f8_map(a, s.M, s.K, ld_a, BN), s, status);
+}
+
+// Row-major outputs [rows, cols] with row stride ld, boxes of 32 rows x 128
+// bytes with the 128-byte swizzle; stores past the end are dropped.
+CUtensorMap out_map(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int dtype) {
+  CUtensorMap m;
+  const int es = elem_bytes(dtype);
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * es};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType t = dtype == VDK_FP32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == VDK_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = encode_fn()(&m, t, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(VD_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")");
+  return m;
+}
+
+template <class O>
+void launch_f8_pair(const void* a, int64_t ld_a, const void* w, int64_t ld_w, const F8Shape& s, int dtype, int* status,
+                    cudaStream_t stream) {
+  using Cfg = F8PairConfig;
+  auto kernel = fp8_gemm_pair_kernel<O>;
+  cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES),
+             "shared memory size");
+  cudaFuncAttributes attr;
+  cuda_check(cudaFuncGetAttributes(&attr, kernel), "kernel attributes");
+  if (attr.numRegs != Cfg::LAUNCH_REGS) fail(VD_ECUDA, "fp8_gemm_pair_kernel was built with another register count");
+  const int tiles = ((s.M + 255) / 256) * ((s.N + 255) / 256);
+  const int grid = 2 * std::min(tiles, sm_count() / 2);
+  kernel<<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(
+      f8_map(a, s.M, s.K, ld_a, 128), f8_map(w, s.N, s.K, ld_w, 128),
+      s.out_aligned ? out_map(s.out, s.M, s.N, s.ld_out, dtype) : CUtensorMap{}, s, status);
+  launched();
 }
 
 }  // namespace
@@ -200,9 +235,11 @@ extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     by_type(out_dtype, [&](auto tag) {
       using O = decltype(tag);
-      if (M <= 32) launch_f8<true, 32, O>(a, ld_a, w, ld_w, s, status, st);
-      else if (M <= 64) launch_f8<true, 64, O>(a, ld_a, w, ld_w, s, status, st);
-      else launch_f8<false, 128, O>(a, ld_a, w, ld_w, s, status, st);
+      if (M <= 16) launch_f8_rows<16, O>(a, ld_a, w, ld_w, s, status, st);
+      else if (M <= 32) launch_f8_rows<32, O>(a, ld_a, w, ld_w, s, status, st);
+      else if (M <= 64) launch_f8_rows<64, O>(a, ld_a, w, ld_w, s, status, st);
+      else if (M <= 128) launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, status, st);
+      else launch_f8_pair<O>(a, ld_a, w, ld_w, s, out_dtype, status, st);
     });
   });
 }
