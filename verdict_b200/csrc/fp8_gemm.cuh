@@ -28,6 +28,7 @@ struct F8Shape {
   int64_t ld_out;
   int out_aligned;  // rows of out start on 16 bytes
   int splits;       // CTAs along K: the cluster's size
+  int stages;       // of the shared-memory ring (fp8_gemm_rows_kernel)
 };
 
 // mbar_wait with the clock read only after a run of polls: reading the global
@@ -126,6 +127,8 @@ template <int BN>
 struct F8RowsConfig {
   static constexpr int BM = 128;
   static constexpr int BK = 128;
+  // Ring depth: with two CTAs on an SM, and for one that has it to itself.
+  static constexpr int SHARED_STAGES = BN == 128 ? 0 : BN == 64 ? 3 : 4;
   static constexpr int STAGES = BN == 128 ? 4 : BN == 64 ? 6 : 8;
   static constexpr int W_BYTES = BM * BK;
   static constexpr int A_BYTES = BN * BK;
@@ -134,31 +137,36 @@ struct F8RowsConfig {
   static constexpr int TMEM_COLS = BUFS * BN;
   static constexpr int DRAIN_WARPS = BN >= 64 ? 8 : 4;
   static constexpr int COLS = BN / (DRAIN_WARPS / 4);  // columns of a drain warp
-  static constexpr int SCALE_KB = 16;
+  static constexpr int SCALE_KB = BN >= 64 ? 8 : 16;   // k-blocks of scales staged at a time
   static constexpr int SCALE_BYTES = 2 * SCALE_KB * BN * 4;
-  static constexpr int MAX_SPLITS = 8;
-  static constexpr int SUM_BYTES = (BN + MAX_SPLITS) * BM * 4;  // what the cluster's CTAs send here
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + SCALE_BYTES + SUM_BYTES + 512;
+  static constexpr int MAX_SPLITS = BN >= 32 ? 8 : BN / 4;  // shares of at least four columns
+  static constexpr int SUM_BYTES = BN * BM * 4;  // what the cluster's CTAs send here
+  // Up to 64 tokens two CTAs may share an SM: one's latencies hide under the other.
+  static constexpr int CTAS_PER_SM = SHARED_STAGES > 0 ? 2 : 1;
+  static constexpr int smem_bytes(int stages, int splits) {
+    return 1024 + stages * STAGE_BYTES + 512 + SCALE_BYTES + (splits > 1 ? SUM_BYTES : 0);
+  }
   static constexpr int THREADS = 64 + 32 * DRAIN_WARPS;
 };
 
 template <int BN, class O>
-__global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
+__global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::CTAS_PER_SM)
     fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, F8Shape s,
                          int* err) {
   using Cfg = F8RowsConfig<BN>;
-  constexpr int BM = Cfg::BM, BK = Cfg::BK, STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, COLS = Cfg::COLS;
+  constexpr int BM = Cfg::BM, BK = Cfg::BK, BUFS = Cfg::BUFS, COLS = Cfg::COLS;
   constexpr int DRAIN = 32 * Cfg::DRAIN_WARPS;
+  const int stages = s.stages;
   constexpr uint32_t IDESC = umma_idesc_f8(BM, BN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
-  uint8_t* sA = smem + STAGES * Cfg::W_BYTES;
-  float* sScale = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);
-  float* sSum = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALE_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALE_BYTES + Cfg::SUM_BYTES);
-  uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;
+  uint8_t* sA = smem + stages * Cfg::W_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * Cfg::STAGE_BYTES);
+  float* sScale = reinterpret_cast<float*>(smem + stages * Cfg::STAGE_BYTES + 512);
+  float* sSum = reinterpret_cast<float*>(smem + stages * Cfg::STAGE_BYTES + 512 + Cfg::SCALE_BYTES);  // splits > 1
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
   uint64_t* acc_empty = acc_full + BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + BUFS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -174,7 +182,9 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
   const int kb1 = static_cast<int>(static_cast<int64_t>(kblocks) * (part + 1) / s.splits);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmA);
+    for (int i = 0; i < stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -208,12 +218,12 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
         mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
         tma_load_2d(sW + stage * Cfg::W_BYTES, &tmW, &full[stage], kb * BK, n0);
         tma_load_2d(sA + stage * Cfg::A_BYTES, &tmA, &full[stage], kb * BK, m0);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
+        if (++stage == stages) stage = 0, phase ^= 1;
       }
       // Every load has landed and been consumed before the CTA may exit.
-      for (int i = 0; i < STAGES && ok; ++i) {
+      for (int i = 0; i < stages && ok; ++i) {
         ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
+        if (++stage == stages) stage = 0, phase ^= 1;
       }
     }
     __syncwarp();
@@ -238,7 +248,7 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
         umma_commit(&empty[stage]);
       }
       __syncwarp();
-      if (++stage == STAGES) stage = 0, phase ^= 1;
+      if (++stage == stages) stage = 0, phase ^= 1;
       if (++buf == BUFS) buf = 0, buf_phase ^= 1;
     }
   } else {
@@ -316,20 +326,21 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
         if (m0 + col0 + j < s.M) o[j * s.ld_out] = Elem<O>::from(acc[j] + bias);
     }
   } else {
-    // Column j goes to CTA j / share, into [rank][j % share][row].
-    const int share = (BN + s.splits - 1) / s.splits;
+    // Four columns at a time: column j goes to CTA j / share, there to
+    // [rank][(j % share) / 4][row][4].
+    const int share = BN / s.splits;
     __syncwarp();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA runs
     if (warp >= 2) {
       const int col0 = ((warp - 2) >> 2) * COLS;
-      const uint32_t mine = smem_u32(sSum) + (part * share * BM + row) * 4;
-      int to = col0 / share, at = col0 - to * share;
+      const uint32_t mine = smem_u32(sSum) + (part * share * BM + row * 4) * 4;
 #pragma unroll
-      for (int j = 0; j < COLS; ++j) {
+      for (int j = 0; j < COLS; j += 4) {
+        const int to = (col0 + j) / share, at = (col0 + j) - to * share;
         if (m0 + col0 + j < s.M)
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(mine + at * (BM * 4), to)), "f"(acc[j])
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(mine + at * (BM * 4), to)),
+                       "f"(acc[j]), "f"(acc[j + 1]), "f"(acc[j + 2]), "f"(acc[j + 3])
                        : "memory");
-        if (++at == share) at = 0, ++to;
       }
     }
     __syncwarp();
@@ -337,11 +348,19 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, 1)
     if (warp >= 2 && n < s.N) {
       const float bias = s.bias ? __ldg(s.bias + n) : 0.0f;
       const int first = part * share;
-      const int count = min(min(share, BN - first), s.M - m0 - first);
-      for (int j = (warp - 2) >> 2; j < count; j += Cfg::DRAIN_WARPS / 4) {
-        float v = 0.0f;
-        for (int r = 0; r < s.splits; ++r) v += sSum[(r * share + j) * BM + row];
-        out[static_cast<int64_t>(m0 + first + j) * s.ld_out + n] = Elem<O>::from(v + bias);
+      const int count = min(share, s.M - m0 - first);
+      const float4* sums = reinterpret_cast<const float4*>(sSum) + row;
+      for (int j = ((warp - 2) >> 2) * 4; j < count; j += Cfg::DRAIN_WARPS) {
+        float v[4] = {bias, bias, bias, bias};
+#pragma unroll 4
+        for (int r = 0; r < s.splits; ++r) {
+          const float4 x = sums[(r * share + j) * (BM / 4)];
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        O* o = out + static_cast<int64_t>(m0 + first + j) * s.ld_out + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i < count) o[i * s.ld_out] = Elem<O>::from(v[i]);
       }
     }
   }

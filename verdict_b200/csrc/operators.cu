@@ -2,9 +2,12 @@
 // argument checks, the choice of a kernel variant and the launch on the
 // caller's stream.  Nothing here allocates or waits.
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "vdexec_kernels.h"
 
@@ -89,22 +92,70 @@ CUtensorMap f8_map(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int 
   return m;
 }
 
+// Clusters of `splits` CTAs of fp8_gemm_rows_kernel that the device holds at
+// once, one CTA on an SM (what the occupancy call assumes of kernels that use
+// tensor memory; two were seen to run); asked once per device and kernel.
 template <int BN, class O>
-void launch_f8_rows(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8Shape s, int* status,
-                    cudaStream_t stream) {
+int f8_rows_clusters(int splits) {
   using Cfg = F8RowsConfig<BN>;
-  auto kernel = fp8_gemm_rows_kernel<BN, O>;
-  cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES),
-             "shared memory size");
-  const int n_tiles = (s.N + 127) / 128, m_tiles = (s.M + BN - 1) / BN;
-  // K is split while the CTAs still fit on the GPU at once (one per SM) and
-  // each keeps at least four k-blocks.
+  static std::atomic<int> known[64][4];
+  int dev = 0;
+  cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (dev < 0 || dev >= 64) fail(VD_EINVAL, "device index out of range");
+  std::atomic<int>& slot = known[dev][splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    auto kernel = fp8_gemm_rows_kernel<BN, O>;
+    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    Cfg::smem_bytes(Cfg::STAGES, Cfg::MAX_SPLITS)),
+               "shared memory size");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(splits * 1024);
+    cfg.blockDim = dim3(Cfg::THREADS);
+    cfg.dynamicSmemBytes = Cfg::smem_bytes(Cfg::STAGES, splits);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cuda_check(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg), "cluster occupancy");
+    slot.store(n = std::max(n, 1), std::memory_order_relaxed);
+  }
+  return n;
+}
+
+struct F8RowsPlan {
+  int splits, stages;
+  int steps;  // k-blocks that the last CTA to finish goes through, one after another
+};
+
+template <int BN, class O>
+F8RowsPlan plan_f8_rows(const F8Shape& s) {
+  using Cfg = F8RowsConfig<BN>;
   const int kblocks = (s.K + 127) / 128;
-  const int tiles = n_tiles * m_tiles;
-  s.splits = 1;
-  while (s.splits < Cfg::MAX_SPLITS && tiles * (s.splits + 1) <= sm_count() && kblocks / (s.splits + 1) >= 4) ++s.splits;
-  launch_cluster(kernel, dim3(n_tiles * s.splits, m_tiles), Cfg::THREADS, Cfg::SMEM_BYTES, s.splits, stream,
-                 f8_map(w, s.N, s.K, ld_w, 128), f8_map(a, s.M, s.K, ld_a, BN), s, status);
+  const int tiles = ((s.N + 127) / 128) * ((s.M + BN - 1) / BN);
+  // The most CTAs per tile that still run at once, each with at least four
+  // k-blocks: a second wave costs more than the split gains.
+  F8RowsPlan p{Cfg::MAX_SPLITS, 0, 0};
+  int room = f8_rows_clusters<BN, O>(p.splits);
+  while (p.splits > 1 && (kblocks / p.splits < 4 || tiles > Cfg::CTAS_PER_SM * room))
+    room = f8_rows_clusters<BN, O>(p.splits /= 2);
+  p.stages = Cfg::CTAS_PER_SM == 1 || tiles <= room ? Cfg::STAGES : Cfg::SHARED_STAGES;
+  p.steps = (tiles + room - 1) / room * ((kblocks + p.splits - 1) / p.splits);
+  return p;
+}
+
+template <int BN, class O>
+void launch_f8_rows(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8Shape s, const F8RowsPlan& plan,
+                    int* status, cudaStream_t stream) {
+  using Cfg = F8RowsConfig<BN>;
+  s.splits = plan.splits;
+  s.stages = plan.stages;
+  const int n_tiles = (s.N + 127) / 128, m_tiles = (s.M + BN - 1) / BN;
+  launch_cluster(fp8_gemm_rows_kernel<BN, O>, dim3(n_tiles * s.splits, m_tiles), Cfg::THREADS,
+                 Cfg::smem_bytes(s.stages, s.splits), s.splits, stream, f8_map(w, s.N, s.K, ld_w, 128),
+                 f8_map(a, s.M, s.K, ld_a, BN), s, status);
 }
 
 // Row-major outputs [rows, cols] with row stride ld, boxes of 32 rows x 128
@@ -235,10 +286,23 @@ extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     by_type(out_dtype, [&](auto tag) {
       using O = decltype(tag);
-      if (M <= 16) launch_f8_rows<16, O>(a, ld_a, w, ld_w, s, status, st);
-      else if (M <= 32) launch_f8_rows<32, O>(a, ld_a, w, ld_w, s, status, st);
-      else if (M <= 64) launch_f8_rows<64, O>(a, ld_a, w, ld_w, s, status, st);
-      else if (M <= 128) launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, status, st);
+      auto rows = [&](auto bn) {
+        constexpr int BN = decltype(bn)::value;
+        launch_f8_rows<BN, O>(a, ld_a, w, ld_w, s, plan_f8_rows<BN, O>(s), status, st);
+      };
+      if (M <= 16) return rows(std::integral_constant<int, 16>());
+      if (M <= 32) return rows(std::integral_constant<int, 32>());
+      if (M <= 64) return rows(std::integral_constant<int, 64>());
+      // A pair goes through a k-block of a 256 x 256 tile in 0.53 us, a CTA of
+      // the other kernel through one of a 128 x 128 tile in 0.6, but it can split
+      // K, for about four k-blocks' time (bf16, us, pairs / rows: 128 x 6144 x
+      // 4096 19.4 / 14.8, 100 x 4096 x 12288 46.8 / 19.0, 200 x 4096 x 4096 19.1
+      // / 14.8; 256 x 6144 x 4096 19.5 / 21.2, 100 x 24576 x 4096 36.0 / 41.1).
+      const int pairs = sm_count() / 2;
+      const int pair_tiles = ((s.M + 255) / 256) * ((s.N + 255) / 256);
+      const int pair_steps = (pair_tiles + pairs - 1) / pairs * ((s.K + 127) / 128);
+      const F8RowsPlan plan = plan_f8_rows<128, O>(s);
+      if (plan.steps * 1.1 + 4 < pair_steps) launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, plan, status, st);
       else launch_f8_pair<O>(a, ld_a, w, ld_w, s, out_dtype, status, st);
     });
   });
