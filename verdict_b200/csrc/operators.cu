@@ -520,11 +520,11 @@ extern "C" VD_API int vdk_token_logprobs(const void* logits, int64_t ld, int64_t
     p.top = top;
     p.inv_temperature = 1.0f / temperature;
     p.logprobs = logprobs, p.entropy = entropy, p.lse = lse, p.top_ids = top_ids, p.top_logprobs = top_logprobs;
-    // CTAs share a row while that leaves at most two per SM and each keeps a
-    // batch of loads (kLpThreads * kLpUnroll * 16 bytes) or so.
+    // CTAs share a row until all can run, while each keeps a batch of loads
+    // (kLpThreads * kLpUnroll * 16 bytes).
     p.splits = 1;
     const int64_t bytes = vocab * elem_bytes(dtype);
-    while (p.splits < kLpMaxSplits && rows * p.splits * 2 <= 2 * sm_count() && bytes / (p.splits * 2) >= 16384)
+    while (p.splits < kLpMaxSplits && rows * p.splits < kLpCtasPerSm * sm_count() && bytes / (p.splits * 2) >= 16384)
       p.splits *= 2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     by_type(dtype, [&](auto tag) {

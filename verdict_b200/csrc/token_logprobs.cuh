@@ -22,6 +22,8 @@
 // distributed shared memory.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm2.cuh"
 #include "row_io.cuh"
 
@@ -43,9 +45,11 @@ struct LogprobParams {
   int splits;           // CTAs of a row: the cluster's size
 };
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
+constexpr int kLpCtasPerSm = 4;
 constexpr int kLpUnroll = 4;        // 16-byte loads in flight per thread
-constexpr int kLpGroups = kLpThreads / 8;
+constexpr int kLpGroups = 64;
+constexpr int kLpGroupSize = kLpThreads / kLpGroups;
 constexpr int kLpMaxTop = kLpGroups;
 constexpr int kLpCap = 1024;        // candidates
 constexpr int kLpMaxSplits = 8;
@@ -105,52 +109,88 @@ __device__ __forceinline__ LpStats lp_join_lanes(LpStats a, float c, int width) 
   return a;
 }
 
+// 16 bytes of a row: slot v, counted from the row's start rounded down to 16
+// bytes, holds entries v * VEC - skew and on; -inf outside the row.
+template <class T>
+__device__ __forceinline__ uint4 lp_load(const T* row, int vocab, int skew, int v, int end) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int at = v * VEC - skew;
+  if (v < end && at >= 0 && at + VEC <= vocab) return __ldg(reinterpret_cast<const uint4*>(row + at));
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      w[j] = v < end && at + j >= 0 && at + j < vocab ? __float_as_uint(row[at + j]) : 0xff800000u;
+    } else {
+      const unsigned short* s = reinterpret_cast<const unsigned short*>(row);
+      const uint32_t none = Elem<T>::kUmmaFormat == 1 ? 0xff80u : 0xfc00u;  // -inf
+      const int e = at + 2 * j;
+      const uint32_t lo = v < end && e >= 0 && e < vocab ? s[e] : none;
+      const uint32_t hi = v < end && e + 1 >= 0 && e + 1 < vocab ? s[e + 1] : none;
+      w[j] = lo | (hi << 16);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <class T>
+__device__ __forceinline__ void lp_unpack(uint4 r, float (&x)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      x[j] = __uint_as_float(w[j]);
+    } else {
+      const float2 f = Elem<T>::unpack2(w[j]);
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
+    }
+  }
+}
+
 template <class T>
 struct LpBatch {
   static constexpr int VEC = 16 / sizeof(T);
   uint4 r[kLpUnroll];
 
-  // Slots of 16 bytes counted from the row's start rounded down to 16 bytes;
-  // slot v holds elements v * VEC - skew ..  Edge slots are filled with -inf
-  // outside the row.
-  __device__ __forceinline__ void load(const T* row, int vocab, int skew, int slot, int end) {
+  __device__ __forceinline__ void load(const T* row, int vocab, int skew, int base, int end) {
+    const int slot = base + static_cast<int>(threadIdx.x);
+    // Inside the row and the CTA's part of it: no checks per load.
+    if (base > 0 && base + kLpThreads * kLpUnroll < end) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + (static_cast<int64_t>(slot) * VEC - skew));
 #pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) {
-      const int v = slot + k * kLpThreads;
-      const int at = v * VEC - skew;
-      if (v < end && at >= 0 && at + VEC <= vocab) {
-        r[k] = __ldg(reinterpret_cast<const uint4*>(row + at));
-      } else {
-        uint32_t w[4];
+      for (int k = 0; k < kLpUnroll; ++k) r[k] = __ldg(p + k * kLpThreads);
+      return;
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (sizeof(T) == 4) {
-            w[j] = v < end && at + j >= 0 && at + j < vocab ? __float_as_uint(row[at + j]) : 0xff800000u;
-          } else {
-            const unsigned short* s = reinterpret_cast<const unsigned short*>(row);
-            const uint32_t none = Elem<T>::kUmmaFormat == 1 ? 0xff80u : 0xfc00u;  // -inf
-            const int e = at + 2 * j;
-            const uint32_t lo = v < end && e >= 0 && e < vocab ? s[e] : none;
-            const uint32_t hi = v < end && e + 1 >= 0 && e + 1 < vocab ? s[e + 1] : none;
-            w[j] = lo | (hi << 16);
-          }
-        }
-        r[k] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+    for (int k = 0; k < kLpUnroll; ++k) r[k] = lp_load(row, vocab, skew, slot + k * kLpThreads, end);
+  }
+  // The largest entry of load u (NaN is passed over), two 16-bit entries at a time.
+  __device__ __forceinline__ float largest(int u) const {
+    if constexpr (sizeof(T) == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(&r[u]);
+      return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+    } else {
+      using T2 = typename std::conditional<Elem<T>::kUmmaFormat == 1, __nv_bfloat162, __half2>::type;
+      const T2* v = reinterpret_cast<const T2*>(&r[u]);
+      const T2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+      const float2 f = Elem<T>::unpack2(*reinterpret_cast<const uint32_t*>(&m));
+      return fmaxf(f.x, f.y);
     }
   }
-  __device__ __forceinline__ void get(int k, float (&x)[VEC]) const {
-    const uint32_t w[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+  // Bit u * VEC + j for each entry of at least `low` (which is above -inf).
+  __device__ __forceinline__ uint32_t reaching(const float (&top)[kLpUnroll], float low) const {
+    uint32_t bits = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        x[j] = __uint_as_float(w[j]);
-      } else {
-        const float2 f = Elem<T>::unpack2(w[j]);
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
+    for (int u = 0; u < kLpUnroll; ++u) {
+      if (top[u] >= low) {
+        float v[VEC];
+        lp_unpack<T>(r[u], v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) bits |= v[j] >= low ? 1u << (u * VEC + j) : 0u;
       }
     }
+    return bits;
   }
 };
 
@@ -167,23 +207,26 @@ struct LpShared {
   LpStats total;
 };
 
-// The k-th largest of the 64 groups' largest keys (a group is eight threads):
+// The k-th largest of the 64 groups' largest keys (a group is kLpGroupSize threads):
 // at least k entries reach it.  0 where fewer groups have an entry.
 __device__ __forceinline__ uint64_t lp_group_bound(LpShared& sh, uint64_t best, int k) {
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
+  for (int o = kLpGroupSize / 2; o > 0; o >>= 1) {
     const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
     best = b > best ? b : best;
   }
-  if ((threadIdx.x & 7) == 0) sh.group[threadIdx.x >> 3] = best;
+  const int group = threadIdx.x / kLpGroupSize, in_group = threadIdx.x % kLpGroupSize;
+  if (in_group == 0) sh.group[group] = best;
   if (threadIdx.x == 0) sh.bound = 0;
   __syncthreads();
-  if (threadIdx.x < kLpGroups) {
-    const uint64_t mine = sh.group[threadIdx.x];
-    int larger = 0;
-    for (int i = 0; i < kLpGroups; ++i) larger += sh.group[i] > mine;
-    if (larger == k - 1 && mine != 0) sh.bound = mine;  // keys are distinct
-  }
+  // A group's threads count the keys above its own.
+  const uint64_t mine = sh.group[group];
+  int larger = 0;
+#pragma unroll
+  for (int i = 0; i < kLpGroups; i += kLpGroupSize) larger += sh.group[i + in_group] > mine;
+#pragma unroll
+  for (int o = kLpGroupSize / 2; o > 0; o >>= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+  if (larger == k - 1 && mine != 0) sh.bound = mine;  // keys are distinct
   __syncthreads();
   return sh.bound;
 }
@@ -211,7 +254,7 @@ __device__ __forceinline__ void lp_select(LpShared& sh, int n, int k) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LogprobParams p) {
+__global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kernel(LogprobParams p) {
   using Batch = LpBatch<T>;
   constexpr int VEC = Batch::VEC;
   extern __shared__ __align__(16) uint8_t lp_smem[];
@@ -228,70 +271,74 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LogprobParam
   const int k = p.top;
 
   LpStats st{-INFINITY, 0.0f, 0.0f};
+  int batches = 0;
   uint64_t bound = 0;
-  float bound_x = -INFINITY;
+  float bound_x = -3.402823466e38f;  // every entry but -inf
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  // Entries at or above the bound; -inf (and NaN) are never listed.
-  auto collect = [&](const Batch& b, int slot) {
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      float v[VEC];
-      b.get(u, v);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (v[j] >= bound_x && v[j] > -INFINITY) {
-          const uint64_t key = lp_key(v[j], static_cast<uint32_t>((slot + u * kLpThreads) * VEC - skew + j));
-          if (key >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kLpCap) sh.cand[at] = key;
-          }
-        }
+  auto id_of = [&](int slot, int bit) { return (slot + bit / VEC * kLpThreads) * VEC - skew + bit % VEC; };
+  // Entries at or above the bound go to the buffer.
+  auto collect = [&](const Batch& b, const float (&top)[kLpUnroll], int slot) {
+    uint32_t bits = b.reaching(top, bound_x);
+#pragma unroll 1
+    while (bits) {
+      const int id = id_of(slot, __ffs(bits) - 1);
+      bits &= bits - 1;
+      const uint64_t key = lp_key(Elem<T>::to(x[id]), static_cast<uint32_t>(id));
+      if (key >= bound) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kLpCap) sh.cand[at] = key;
       }
     }
   };
   for (int base = begin; base < end; base += kLpThreads * kLpUnroll) {
     Batch b;
-    b.load(x, p.vocab, skew, base + tid, end);
-    float bm = -INFINITY;
+    b.load(x, p.vocab, skew, base, end);
+    float top[kLpUnroll];
 #pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      float v[VEC];
-      b.get(u, v);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) bm = fmaxf(bm, v[j]);
-    }
+    for (int u = 0; u < kLpUnroll; ++u) top[u] = b.largest(u);
+    static_assert(kLpUnroll == 4, "");
+    const float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     if (bm > st.m) st = lp_rescale(st, bm, c);
     const float m = st.m == -INFINITY ? 0.0f : st.m;
+    // Two running pairs (even and odd entries), joined at the batch's end.
+    float2 sum = make_float2(st.s, 0.0f), mom = make_float2(st.u, 0.0f);
+    const float2 neg_m = make_float2(-m, -m), cc = make_float2(c, c);
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
       float v[VEC];
-      b.get(u, v);
+      lp_unpack<T>(b.r[u], v);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float t = max_nan((v[j] - m) * c, kLpFloor);
-        const float e = exp2_approx(t);
-        st.s += e;
-        st.u = fmaf(e, t, st.u);
+      for (int j = 0; j < VEC; j += 2) {
+        float2 t = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), neg_m), cc);
+        t.x = max_nan(t.x, kLpFloor);
+        t.y = max_nan(t.y, kLpFloor);
+        const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+        sum = __fadd2_rn(sum, e);
+        mom = __ffma2_rn(e, t, mom);
       }
     }
+    st.s = sum.x + sum.y;
+    st.u = mom.x + mom.y;
     if (k > 0) {
       if (base == begin) {
+        // The thread's largest entry, the first of equal ones.
         uint64_t best = 0;
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
-          float v[VEC];
-          b.get(u, v);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const uint64_t key = lp_key(v[j], static_cast<uint32_t>((base + tid + u * kLpThreads) * VEC - skew + j));
-            if (v[j] > -INFINITY && key > best) best = key;
-          }
-        }
+        if (bm > -INFINITY) best = lp_key(bm, static_cast<uint32_t>(id_of(base + tid, __ffs(b.reaching(top, bm)) - 1)));
         bound = lp_group_bound(sh, best, k);
         if (bound) bound_x = lp_key_value(bound);
       }
-      if (bm >= bound_x) collect(b, base + tid);
+      if (bm >= bound_x) collect(b, top, base + tid);
+      // After 2, 4, 8 .. batches the bound rises with the maxima so far (their
+      // ids are not kept: the key of any entry with that value will do), so
+      // that each doubling of what has been read adds about k candidates.
+      if (++batches > 1 && (batches & (batches - 1)) == 0) {
+        const uint64_t higher = lp_group_bound(sh, st.m > -INFINITY ? lp_key(st.m, 0xffffffffu - tid) : 0, k);
+        if (higher != 0 && (higher | 0xffffffffu) > (bound | 0xffffffffu)) {
+          bound = higher & ~0xffffffffull;
+          bound_x = lp_key_value(bound);
+        }
+      }
     }
   }
 
@@ -315,17 +362,16 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LogprobParam
         for (int i = tid; i < 256; i += kLpThreads) sh.hist[i] = 0;
         __syncthreads();
         for (int base = begin; base < end; base += kLpThreads * kLpUnroll) {
-          Batch b;
-          b.load(x, p.vocab, skew, base + tid, end);
 #pragma unroll 1
           for (int u = 0; u < kLpUnroll; ++u) {
+            const int slot = base + tid + u * kLpThreads;
             float v[VEC];
-            b.get(u, v);
+            lp_unpack<T>(lp_load(x, p.vocab, skew, slot, end), v);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-              const uint64_t key = lp_key(v[j], static_cast<uint32_t>((base + tid + u * kLpThreads) * VEC - skew + j));
-              const bool in = shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8));
-              if (v[j] > -INFINITY && in) atomicAdd(&sh.hist[(key >> shift) & 255], 1);
+              const uint64_t key = lp_key(v[j], static_cast<uint32_t>(slot * VEC - skew + j));
+              if (v[j] > -INFINITY && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
+                atomicAdd(&sh.hist[(key >> shift) & 255], 1);
             }
           }
         }
@@ -346,13 +392,16 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LogprobParam
       }
       bound = prefix;
       bound_x = lp_key_value(bound);
-      if (!(bound_x >= -INFINITY)) bound_x = -INFINITY;  // a prefix can fall outside the numbers
+      if (!(bound_x >= -3.402823466e38f)) bound_x = -3.402823466e38f;  // a prefix can lie below every number
       if (tid == 0) sh.count = 0;
       __syncthreads();
       for (int base = begin; base < end; base += kLpThreads * kLpUnroll) {
         Batch b;
-        b.load(x, p.vocab, skew, base + tid, end);
-        collect(b, base + tid);
+        b.load(x, p.vocab, skew, base, end);
+        float top[kLpUnroll];
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) top[u] = b.largest(u);
+        collect(b, top, base + tid);
       }
       __syncthreads();
     }
