@@ -218,24 +218,31 @@ extern "C" VD_API int vdk_quantize_fp8(const void* x, int64_t ld_x, const void* 
     p.ld_x = ld_x, p.ld_gate = ld_gate, p.ld_q = ld_q, p.ld_scale = ld_scale;
     p.blocks = static_cast<uint32_t>(rows * col_blocks);
     p.col_blocks = static_cast<uint32_t>(col_blocks);
+    if (col_blocks > 1) {  // ceil(2^(31 + l) / d), l = ceil(log2 d): exact quotients below 2^31
+      int l = 0;
+      while ((int64_t(1) << l) < col_blocks) ++l;
+      p.div_mul = static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + col_blocks - 1) / col_blocks);
+      p.div_shift = l - 1;
+    }
     p.cols = static_cast<int>(cols);
     p.act = act;
     p.q = static_cast<uint8_t*>(q);
     p.scale = scale;
-    p.q_aligned = (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ld_q % 8 == 0;
     const unsigned per = kQuantUnroll * kQuantThreads / 16;
     const unsigned grid = (p.blocks + per - 1) / per;
+    const bool whole = cols % 8 == 0 && rows16(x, ld_x, dtype) && (!gate || rows16(gate, ld_gate, dtype)) &&
+                       (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ld_q % 8 == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     by_type(dtype, [&](auto tag) {
       using T = decltype(tag);
-      const bool al = rows16(x, ld_x, dtype) && (!gate || rows16(gate, ld_gate, dtype));
-      if (gate) {
-        if (al) quantize_rows_kernel<T, true, true><<<grid, kQuantThreads, 0, s>>>(p);
-        else quantize_rows_kernel<T, true, false><<<grid, kQuantThreads, 0, s>>>(p);
-      } else {
-        if (al) quantize_rows_kernel<T, false, true><<<grid, kQuantThreads, 0, s>>>(p);
-        else quantize_rows_kernel<T, false, false><<<grid, kQuantThreads, 0, s>>>(p);
-      }
+      auto run = [&](auto whole_kernel, auto kernel) {
+        if (whole) whole_kernel<<<grid, kQuantThreads, 0, s>>>(p);
+        else kernel<<<grid, kQuantThreads, 0, s>>>(p);
+      };
+      if (!gate) run(quantize_rows_kernel<T, kGateNone, true>, quantize_rows_kernel<T, kGateNone, false>);
+      else if (act == VDK_ACT_SILU)
+        run(quantize_rows_kernel<T, kGateSilu, true>, quantize_rows_kernel<T, kGateSilu, false>);
+      else run(quantize_rows_kernel<T, kGateAny, true>, quantize_rows_kernel<T, kGateAny, false>);
     });
     launched();
   });

@@ -21,55 +21,75 @@ struct QuantizeParams {
   const void* x;
   const void* gate;
   int64_t ld_x, ld_gate, ld_q, ld_scale;
-  uint32_t blocks, col_blocks;  // rows * col_blocks, ceil(cols / 128)
+  uint32_t blocks, col_blocks;   // rows * col_blocks, ceil(cols / 128)
+  uint32_t div_mul, div_shift;   // id / col_blocks = umulhi(id, div_mul) >> div_shift for ids below 2^31
   int cols, act;
   uint8_t* q;
   float* scale;
-  bool q_aligned;
 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 4;
+constexpr int kQuantUnroll = 2;
 
+__device__ __forceinline__ uint32_t block_row(const QuantizeParams& p, uint32_t id) {
+  return p.div_mul == 0 ? id : __umulhi(id, p.div_mul) >> p.div_shift;
+}
+
+// What multiplies x: the gate's activation, SiLU apart from the others so that
+// the common kernels stay short (fetching instructions was a fifth of their time).
+enum QuantGate : int { kGateNone, kGateSilu, kGateAny };
+
+template <int GATE>
 __device__ __forceinline__ float gate_act(float g, int act) {
-  if (act == kActSilu) return __fdividef(g, 1.0f + __expf(-g));
+  if (GATE == kGateSilu) {  // one exp2 and one reciprocal; the reciprocal of inf is 0
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * r;
+  }
   return apply_act(g, act);
 }
 
-template <class T, bool GATED, bool ALIGNED>
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantizeParams p) {
+// WHOLE: rows of x, gate and q that 8 elements divide and that are aligned for
+// vector access.
+template <class T, int GATE, bool WHOLE>
+__global__ void __launch_bounds__(kQuantThreads, WHOLE && sizeof(T) == 2 ? 6 : 1) quantize_rows_kernel(QuantizeParams p) {
   const int lane16 = threadIdx.x & 15;
   const uint32_t first = blockIdx.x * (kQuantUnroll * kQuantThreads / 16) + (threadIdx.x >> 4);
   Chunk8<T> xr[kQuantUnroll], gr[kQuantUnroll];
 #pragma unroll
   for (int u = 0; u < kQuantUnroll; ++u) {
     const uint32_t id = first + u * (kQuantThreads / 16);
-    const uint32_t row = id / p.col_blocks;
+    const uint32_t row = block_row(p, id);
     const int col = static_cast<int>(id - row * p.col_blocks) * kF8Block + lane16 * 8;
     const int n = id < p.blocks ? p.cols - col : 0;
     const T* x = static_cast<const T*>(p.x) + row * p.ld_x + col;
-    const T* g = GATED ? static_cast<const T*>(p.gate) + row * p.ld_gate + col : nullptr;
-    if (ALIGNED && n >= 8) {
-      xr[u].load(x);
-      if (GATED) gr[u].load(g);
+    const T* g = GATE != kGateNone ? static_cast<const T*>(p.gate) + row * p.ld_gate + col : nullptr;
+    if constexpr (WHOLE) {
+      xr[u].zero();
+      if (GATE != kGateNone) gr[u].zero();
+      if (n > 0) {
+        xr[u].load(x);
+        if (GATE != kGateNone) gr[u].load(g);
+      }
     } else {
       xr[u].load_part(x, n);
-      if (GATED) gr[u].load_part(g, n);
+      if (GATE != kGateNone) gr[u].load_part(g, n);
     }
   }
 #pragma unroll
   for (int u = 0; u < kQuantUnroll; ++u) {
     const uint32_t id = first + u * (kQuantThreads / 16);
-    const uint32_t row = id / p.col_blocks;
+    const uint32_t row = block_row(p, id);
     const uint32_t kb = id - row * p.col_blocks;
     const int col = static_cast<int>(kb) * kF8Block + lane16 * 8;
     float v[8];
     xr[u].get(v);
-    if (GATED) {
+    if (GATE != kGateNone) {
       float g[8];
       gr[u].get(g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= gate_act(g[j], p.act);
+      for (int j = 0; j < 8; ++j) v[j] *= gate_act<GATE>(g[j], p.act);
     }
     uint32_t m = 0;
 #pragma unroll
@@ -77,7 +97,12 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantizePa
     const F8Scale s = f8_scale(max16(m));
     if (id < p.blocks) {
       if (lane16 == 0) p.scale[row * p.ld_scale + kb] = s.scale;
-      f8_store(p.q + row * p.ld_q + col, f8_pack8(v, s.inv), p.cols - col, p.q_aligned);
+      uint8_t* q = p.q + row * p.ld_q + col;
+      if constexpr (WHOLE) {
+        if (col < p.cols) *reinterpret_cast<uint2*>(q) = f8_pack8(v, s.inv);
+      } else {
+        f8_store(q, f8_pack8(v, s.inv), p.cols - col, false);
+      }
     }
   }
 }
