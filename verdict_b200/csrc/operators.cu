@@ -355,14 +355,16 @@ extern "C" VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, c
                                      : kNormOutF8;
     p.residual_scale = residual_scale, p.block_scale = block_scale, p.eps = eps;
     p.gain_add = plus_one ? 1.0f : 0.0f;
-    p.z_aligned = z && (z_dtype == VDK_FP8 ? (reinterpret_cast<uintptr_t>(z) & 7) == 0 && ld_z % 8 == 0
-                                           : rows16(z, ld_z, z_dtype));
-    const bool al = (!y || rows16(y, ld_y, y_dtype)) && (!h || rows16(h, ld_h, h_dtype)) &&
-                    (!h_out || rows16(h_out, ld_h_out, h_dtype)) && aligned16(post_gain) && aligned16(pre_gain) &&
-                    (!gate || gate_col_stride == 0 || rows16(gate, gate_row_stride, gate_dtype));
-    const int chunks = static_cast<int>((cols + 7) / 8);
-    const int nv = chunks <= 256 ? 1 : chunks <= 512 ? 2 : 4;
+    // Four columns a thread and step; few steps for short rows (latency), up to
+    // eight for long ones (at most 512 threads).
+    const int chunks = static_cast<int>((cols + 3) / 4);
+    const int nv = chunks <= 256 ? 1 : chunks <= 512 ? 2 : chunks <= 1280 ? 4 : 8;
     const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+    const bool full =
+        cols == 4ll * nv * threads && (!y || rows16(y, ld_y, y_dtype)) && (!h || rows16(h, ld_h, h_dtype)) &&
+        (!h_out || rows16(h_out, ld_h_out, h_dtype)) && aligned16(post_gain) && aligned16(pre_gain) &&
+        (!gate || gate_col_stride == 0 || rows16(gate, gate_row_stride, gate_dtype)) &&
+        (!z || (z_dtype == VDK_FP8 ? (reinterpret_cast<uintptr_t>(z) & 3) == 0 && ld_z % 4 == 0 : rows16(z, ld_z, z_dtype)));
     const unsigned grid = static_cast<unsigned>(rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     by_type(y_dtype, [&](auto ty) {
@@ -370,14 +372,16 @@ extern "C" VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, c
       auto run = [&](auto th) {
         using TH = decltype(th);
         auto go = [&](auto k) { k<<<grid, threads, 0, s>>>(p); };
-        if (!al) {
+        if (!full) {
           if (nv == 1) go(block_norm_kernel<TY, TH, 1, false>);
           else if (nv == 2) go(block_norm_kernel<TY, TH, 2, false>);
-          else go(block_norm_kernel<TY, TH, 4, false>);
+          else if (nv == 4) go(block_norm_kernel<TY, TH, 4, false>);
+          else go(block_norm_kernel<TY, TH, 8, false>);
         } else {
           if (nv == 1) go(block_norm_kernel<TY, TH, 1, true>);
           else if (nv == 2) go(block_norm_kernel<TY, TH, 2, true>);
-          else go(block_norm_kernel<TY, TH, 4, true>);
+          else if (nv == 4) go(block_norm_kernel<TY, TH, 4, true>);
+          else go(block_norm_kernel<TY, TH, 8, true>);
         }
       };
       if (h_dtype == VDK_FP32) run(float());

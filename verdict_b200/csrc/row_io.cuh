@@ -7,6 +7,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace vd {
@@ -67,6 +69,48 @@ struct Chunk8<float> {
   }
 };
 
+// Four elements: 8 bytes of a 16-bit type, 16 of fp32.  A warp's access is
+// contiguous in either, which eight fp32 elements a thread are not (two
+// accesses of every other 16 bytes: twice the shared L1 wavefronts).
+template <class T>
+struct Chunk4 {
+  typename std::conditional<sizeof(T) == 4, float4, uint2>::type r;
+  __device__ __forceinline__ void zero() {
+    if constexpr (sizeof(T) == 4) r = make_float4(0.f, 0.f, 0.f, 0.f);
+    else r = make_uint2(0, 0);
+  }
+  __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const decltype(r)*>(p); }
+  __device__ __forceinline__ void load_part(const T* p, int n) {
+    if constexpr (sizeof(T) == 4) {
+      r = make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+    } else {
+      const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+      r.x = (n > 0 ? s[0] : 0u) | ((n > 1 ? s[1] : 0u) << 16);
+      r.y = (n > 2 ? s[2] : 0u) | ((n > 3 ? s[3] : 0u) << 16);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[4]) const {
+    if constexpr (sizeof(T) == 4) {
+      v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+    } else {
+      const float2 a = Elem<T>::unpack2(r.x), b = Elem<T>::unpack2(r.y);
+      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+  }
+};
+
+template <bool WHOLE, class T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4], int n) {
+  if constexpr (WHOLE) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack2(v[0], v[1]), Elem<T>::pack2(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = Elem<T>::from(v[j]);
+  }
+}
+
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
@@ -76,13 +120,6 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::pack2(v[0], v[1]), Elem<T>::pack2(v[2], v[3]),
                                               Elem<T>::pack2(v[4], v[5]), Elem<T>::pack2(v[6], v[7]));
   }
-}
-
-template <class T>
-__device__ __forceinline__ void store8_part(T* p, const float (&v)[8], int n) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) p[j] = Elem<T>::from(v[j]);
 }
 
 // |x| as ordered bits: the maximum over these is the largest magnitude, with
@@ -107,13 +144,16 @@ __device__ __forceinline__ F8Scale f8_scale(uint32_t amax_bits) {
   return {__fdiv_rn(a, kF8Max), __fdiv_rn(kF8Max, a)};
 }
 
-// Eight values to e4m3, round to nearest even, saturating (NaN stays NaN).
+// Values to e4m3, round to nearest even, saturating (NaN stays NaN).
+__device__ __forceinline__ uint32_t f8_pack2(float a, float b, float inv) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t f8_pack4(const float (&v)[4], float inv) {
+  return f8_pack2(v[0], v[1], inv) | (f8_pack2(v[2], v[3], inv) << 16);
+}
 __device__ __forceinline__ uint2 f8_pack8(const float (&v)[8], float inv) {
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    w[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  return make_uint2(f8_pack2(v[0], v[1], inv) | (f8_pack2(v[2], v[3], inv) << 16),
+                    f8_pack2(v[4], v[5], inv) | (f8_pack2(v[6], v[7], inv) << 16));
 }
 
 // n < 8 or an unaligned row: byte stores.
