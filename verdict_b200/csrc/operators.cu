@@ -218,12 +218,7 @@ extern "C" VD_API int vdk_quantize_fp8(const void* x, int64_t ld_x, const void* 
     p.ld_x = ld_x, p.ld_gate = ld_gate, p.ld_q = ld_q, p.ld_scale = ld_scale;
     p.blocks = static_cast<uint32_t>(rows * col_blocks);
     p.col_blocks = static_cast<uint32_t>(col_blocks);
-    if (col_blocks > 1) {  // ceil(2^(31 + l) / d), l = ceil(log2 d): exact quotients below 2^31
-      int l = 0;
-      while ((int64_t(1) << l) < col_blocks) ++l;
-      p.div_mul = static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + col_blocks - 1) / col_blocks);
-      p.div_shift = l - 1;
-    }
+    p.per_row = FastDiv(static_cast<uint32_t>(col_blocks));
     p.cols = static_cast<int>(cols);
     p.act = act;
     p.q = static_cast<uint8_t*>(q);
@@ -492,6 +487,11 @@ extern "C" VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_hea
     p.head_dim = head_dim, p.rotary_dim = rotary_dim, p.interleaved = interleaved != 0;
     p.factor = factor;
     p.sin_sign = inverse ? -1.0f : 1.0f;
+    const int width = vec ? 8 : 1;
+    p.rot_units = vec && interleaved ? rotary_dim / 8 : rotary_dim / 2 / width;
+    p.units = p.rot_units + (head_dim - rotary_dim) / width;
+    p.per_token = FastDiv(static_cast<uint32_t>(heads * p.units));
+    p.per_head = FastDiv(static_cast<uint32_t>(p.units));
     const unsigned grid = static_cast<unsigned>((tokens + kRotaryTokens - 1) / kRotaryTokens);
     const size_t smem = kRotaryTokens * (rotary_dim / 2) * sizeof(float2);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

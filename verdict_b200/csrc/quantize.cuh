@@ -22,7 +22,7 @@ struct QuantizeParams {
   const void* gate;
   int64_t ld_x, ld_gate, ld_q, ld_scale;
   uint32_t blocks, col_blocks;   // rows * col_blocks, ceil(cols / 128)
-  uint32_t div_mul, div_shift;   // id / col_blocks = umulhi(id, div_mul) >> div_shift for ids below 2^31
+  FastDiv per_row;               // by col_blocks
   int cols, act;
   uint8_t* q;
   float* scale;
@@ -30,10 +30,6 @@ struct QuantizeParams {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantUnroll = 2;
-
-__device__ __forceinline__ uint32_t block_row(const QuantizeParams& p, uint32_t id) {
-  return p.div_mul == 0 ? id : __umulhi(id, p.div_mul) >> p.div_shift;
-}
 
 // What multiplies x: the gate's activation, SiLU apart from the others so that
 // the common kernels stay short (fetching instructions was a fifth of their time).
@@ -60,7 +56,7 @@ __global__ void __launch_bounds__(kQuantThreads, WHOLE && sizeof(T) == 2 ? 6 : 1
 #pragma unroll
   for (int u = 0; u < kQuantUnroll; ++u) {
     const uint32_t id = first + u * (kQuantThreads / 16);
-    const uint32_t row = block_row(p, id);
+    const uint32_t row = p.per_row(id);
     const int col = static_cast<int>(id - row * p.col_blocks) * kF8Block + lane16 * 8;
     const int n = id < p.blocks ? p.cols - col : 0;
     const T* x = static_cast<const T*>(p.x) + row * p.ld_x + col;
@@ -80,7 +76,7 @@ __global__ void __launch_bounds__(kQuantThreads, WHOLE && sizeof(T) == 2 ? 6 : 1
 #pragma unroll
   for (int u = 0; u < kQuantUnroll; ++u) {
     const uint32_t id = first + u * (kQuantThreads / 16);
-    const uint32_t row = block_row(p, id);
+    const uint32_t row = p.per_row(id);
     const uint32_t kb = id - row * p.col_blocks;
     const int col = static_cast<int>(kb) * kF8Block + lane16 * 8;
     float v[8];

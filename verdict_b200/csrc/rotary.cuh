@@ -34,10 +34,14 @@ struct RotaryParams {
   const uint64_t* turns;  // [rotary_dim / 2]
   int head_dim, rotary_dim, interleaved;
   float factor, sin_sign;
+  // Work units of a head: rotated ones first, then the columns that pass through.
+  int rot_units, units;
+  FastDiv per_token, per_head;  // by heads * units, by units
 };
 
 constexpr int kRotaryTokens = 4;
 constexpr int kRotaryThreads = 256;
+constexpr int kRotaryUnroll = 4;  // units whose loads a thread has in flight
 
 __device__ __forceinline__ float2 rotary_cos_sin(int64_t pos, uint64_t turns) {
   // The top 32 bits of the fraction as a signed number: (-1/2, 1/2] turn.
@@ -70,76 +74,78 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(RotaryParams p) 
   }
   __syncthreads();
   constexpr int W = VEC ? 8 : 1;
-  // Work units of a head: rotated ones first, then the columns that pass through.
-  const int rot_units = (VEC && p.interleaved) ? p.rotary_dim / 8 : half / W;
-  const int copy_units = (p.head_dim - p.rotary_dim) / W;
-  const int units = rot_units + copy_units;
-  const int heads = p.q.heads + p.k.heads;
-  const uint32_t per_token = static_cast<uint32_t>(heads) * units;
-  for (uint32_t w = threadIdx.x; w < nt * per_token; w += kRotaryThreads) {
-    const uint32_t t = w / per_token;
-    uint32_t rest = w - t * per_token;
-    uint32_t head = rest / units;
-    const int u = static_cast<int>(rest - head * units);
-    const bool is_q = head < static_cast<uint32_t>(p.q.heads);
-    const RotaryHeads& r = is_q ? p.q : p.k;
-    if (!is_q) head -= p.q.heads;
-    const T* in = static_cast<const T*>(r.in) + (t0 + t) * r.in_token + head * r.in_head;
-    T* out = static_cast<T*>(r.out) + (t0 + t) * r.out_token + head * r.out_head;
-    const float2* c = cs + t * half;
-    if (u >= rot_units) {
-      const int at = p.rotary_dim + (u - rot_units) * W;
-      if (in + at == out + at) continue;
-      if constexpr (VEC) {
-        Chunk8<T> x;
-        x.load(in + at);
-        x.store(out + at);
-      } else {
-        out[at] = in[at];
-      }
-    } else if (!p.interleaved) {
-      const int at = u * W;
-      if constexpr (VEC) {
-        Chunk8<T> xa, xb;
-        xa.load(in + at);
-        xb.load(in + at + half);
-        float a[8], b[8];
-        xa.get(a);
-        xb.get(b);
+  const uint32_t heads = p.q.heads + p.k.heads;
+  const uint32_t per_token = heads * p.units, total = nt * per_token;
+  using Chunk = typename std::conditional<VEC, Chunk8<T>, T>::type;
+  for (uint32_t w0 = threadIdx.x; w0 < total; w0 += kRotaryThreads * kRotaryUnroll) {
+    const T* in[kRotaryUnroll];
+    T* out[kRotaryUnroll];
+    int unit[kRotaryUnroll], first[kRotaryUnroll];
+    Chunk a[kRotaryUnroll], b[kRotaryUnroll];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 f = c[at + j];
-          const float x = a[j] * f.x - b[j] * f.y;
-          b[j] = b[j] * f.x + a[j] * f.y;
-          a[j] = x;
-        }
-        store8(out + at, a);
-        store8(out + at + half, b);
-      } else {
-        const float2 f = c[at];
-        const float a = Elem<T>::to(in[at]), b = Elem<T>::to(in[at + half]);
-        out[at] = Elem<T>::from(a * f.x - b * f.y);
-        out[at + half] = Elem<T>::from(b * f.x + a * f.y);
-      }
-    } else {
+    for (int i = 0; i < kRotaryUnroll; ++i) {
+      const uint32_t w = w0 + i * kRotaryThreads;
+      if (w >= total) break;
+      const uint32_t t = p.per_token(w), rest = w - t * per_token;
+      uint32_t head = p.per_head(rest);
+      const int u = static_cast<int>(rest - head * p.units);
+      const bool is_q = head < static_cast<uint32_t>(p.q.heads);
+      const RotaryHeads& r = is_q ? p.q : p.k;
+      if (!is_q) head -= p.q.heads;
+      const bool rot = u < p.rot_units;
+      const bool pairs = p.interleaved && !VEC && rot;  // the unit is the neighbours 2u and 2u + 1
+      const int at = rot ? (pairs ? 2 * u : u * W) : p.rotary_dim + (u - p.rot_units) * W;
+      in[i] = static_cast<const T*>(r.in) + (t0 + t) * r.in_token + head * r.in_head + at;
+      out[i] = static_cast<T*>(r.out) + (t0 + t) * r.out_token + head * r.out_head + at;
+      unit[i] = u;
+      first[i] = static_cast<int>(t) * half;  // of the token's cosines and sines
+      const int other = pairs ? 1 : half;     // from a to b
+      const bool two = rot && (pairs || !p.interleaved);
       if constexpr (VEC) {
-        Chunk8<T> x;
-        x.load(in + u * 8);
+        a[i].load(in[i]);
+        if (two) b[i].load(in[i] + other);
+      } else {
+        a[i] = *in[i];
+        if (two) b[i] = in[i][other];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRotaryUnroll; ++i) {
+      if (w0 + i * kRotaryThreads >= total) break;
+      const float2* c = cs + first[i];
+      if (unit[i] >= p.rot_units) {
+        if (in[i] == out[i]) continue;
+        if constexpr (VEC) a[i].store(out[i]);
+        else *out[i] = a[i];
+      } else if constexpr (!VEC) {
+        const float2 f = c[unit[i]];
+        const float x = Elem<T>::to(a[i]), y = Elem<T>::to(b[i]);
+        out[i][0] = Elem<T>::from(x * f.x - y * f.y);
+        out[i][p.interleaved ? 1 : half] = Elem<T>::from(y * f.x + x * f.y);
+      } else if (p.interleaved) {
         float v[8];
-        x.get(v);
+        a[i].get(v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 f = c[u * 4 + j];
-          const float a = v[2 * j], b = v[2 * j + 1];
-          v[2 * j] = a * f.x - b * f.y;
-          v[2 * j + 1] = b * f.x + a * f.y;
+          const float2 f = c[unit[i] * 4 + j];
+          const float x = v[2 * j], y = v[2 * j + 1];
+          v[2 * j] = x * f.x - y * f.y;
+          v[2 * j + 1] = y * f.x + x * f.y;
         }
-        store8(out + u * 8, v);
+        store8(out[i], v);
       } else {
-        const float2 f = c[u];
-        const float a = Elem<T>::to(in[2 * u]), b = Elem<T>::to(in[2 * u + 1]);
-        out[2 * u] = Elem<T>::from(a * f.x - b * f.y);
-        out[2 * u + 1] = Elem<T>::from(b * f.x + a * f.y);
+        float x[8], y[8];
+        a[i].get(x);
+        b[i].get(y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2 f = c[unit[i] * 8 + j];
+          const float r = x[j] * f.x - y[j] * f.y;
+          y[j] = y[j] * f.x + x[j] * f.y;
+          x[j] = r;
+        }
+        store8(out[i], x);
+        store8(out[i] + half, y);
       }
     }
   }

@@ -19,6 +19,21 @@ struct Elem<float> {
   __device__ __forceinline__ static float to(float x) { return x; }
 };
 
+// Division of numbers below 2^31 by one fixed on the host: ceil(2^(31 + l) / d)
+// with l = ceil(log2 d) gives exact quotients.
+struct FastDiv {
+  uint32_t mul = 0, shift = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t d) {
+    if (d <= 1) return;
+    uint32_t l = 0;
+    while ((uint64_t(1) << l) < d) ++l;
+    mul = static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return mul == 0 ? n : __umulhi(n, mul) >> shift; }
+};
+
 template <class T>
 struct Chunk8 {
   uint4 r;
