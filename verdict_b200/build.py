@@ -10,6 +10,7 @@ no libcuda at link time.
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -24,6 +25,9 @@ SOURCES = [os.path.join(CSRC, "vdexec.cu"), os.path.join(CSRC, "operators.cu")]
 DEPS = ([os.path.join(CSRC, f) for f in os.listdir(CSRC)]
         + [os.path.join(INCLUDE, "vdexec.h"), os.path.join(INCLUDE, "vdexec_kernels.h")])
 OBJ = os.path.join(PKG, "_build")
+# The torch binding of verdict_b200/ops.py, built beside the library where torch is installed.
+TORCH_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_LIB = os.path.join(PKG, "_torch_ops.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -44,7 +48,37 @@ def up_to_date() -> bool:
     if not os.path.exists(LIB):
         return False
     t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(p) <= t for p in DEPS if os.path.exists(p))
+    return all(os.path.getmtime(p) <= t for p in DEPS if os.path.exists(p) and p != TORCH_SOURCE)
+
+
+def torch_up_to_date() -> bool:
+    if not os.path.exists(TORCH_LIB):
+        return False
+    t = os.path.getmtime(TORCH_LIB)
+    return all(os.path.getmtime(p) <= t for p in (TORCH_SOURCE, os.path.join(INCLUDE, "vdexec_kernels.h")))
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
+    """Compile verdict_b200/_torch_ops.so against the installed torch; it links libvdexec.so beside it."""
+    if not force and torch_up_to_date():
+        return TORCH_LIB
+    import sysconfig
+
+    from torch.utils import cpp_extension
+    import torch
+
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", INCLUDE,
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    for path in cpp_extension.include_paths():
+        cmd += ["-isystem", path]
+    for path in cpp_extension.library_paths():
+        cmd += ["-L", path]
+    cmd += [TORCH_SOURCE, "-o", TORCH_LIB + ".tmp", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            "-L", PKG, "-l:libvdexec.so", "-Wl,-rpath,$ORIGIN"]
+    _run(cmd, verbose)
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    return TORCH_LIB
 
 
 def _run(cmd: list, verbose: bool) -> None:
@@ -52,7 +86,7 @@ def _run(cmd: list, verbose: bool) -> None:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if verbose:
         print(res.stdout + res.stderr)
 
@@ -72,3 +106,5 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 if __name__ == "__main__":
     print(build(force=True, verbose="--verbose" in sys.argv))
+    if importlib.util.find_spec("torch") is not None:
+        print(build_torch_ops(force=True, verbose="--verbose" in sys.argv))

@@ -62,6 +62,10 @@ void launched() { cuda_check(cudaGetLastError(), "kernel launch"); }
 template <class K, class... Args>
 void launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
                     const Args&... args) {
+  if (cluster == 1) {
+    kernel<<<grid, threads, smem, stream>>>(args...);
+    return launched();
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
