@@ -53,6 +53,7 @@ constexpr int kLpGroupSize = kLpThreads / kLpGroups;
 constexpr int kLpMaxTop = kLpGroups;
 constexpr int kLpCap = 1024;        // candidates
 constexpr int kLpMaxSplits = 8;
+constexpr int kLpInbox = 128;       // candidates a CTA sends on
 // In units of log2: exponents below this are 0 in fp32.
 constexpr float kLpFloor = -1000.0f;
 
@@ -205,6 +206,12 @@ struct LpShared {
   int above;
   LpStats warp[kLpThreads / 32];
   LpStats total;
+  float target_x[kLpThreads];  // each thread its own
+  int target_is[kLpThreads];
+  // What the cluster's CTAs send to its first.
+  LpStats part[kLpMaxSplits];
+  int part_count[kLpMaxSplits];
+  uint64_t inbox[kLpMaxSplits * kLpInbox];
 };
 
 // The k-th largest of the 64 groups' largest keys (a group is kLpGroupSize threads):
@@ -231,14 +238,15 @@ __device__ __forceinline__ uint64_t lp_group_bound(LpShared& sh, uint64_t best, 
   return sh.bound;
 }
 
-// The k largest of n <= kLpCap keys in sh.cand, into sh.best (0 past the last).
-__device__ __forceinline__ void lp_select(LpShared& sh, int n, int k) {
+// The k largest of get(0) .. get(n - 1), n <= kLpCap, into sh.best (0 past the last).
+template <class Get>
+__device__ __forceinline__ void lp_select(LpShared& sh, int n, int k, Get&& get) {
   uint64_t best = 0;
-  for (int i = threadIdx.x; i < n; i += kLpThreads) best = sh.cand[i] > best ? sh.cand[i] : best;
+  for (int i = threadIdx.x; i < n; i += kLpThreads) best = get(i) > best ? get(i) : best;
   if (threadIdx.x == 0) sh.kept_count = 0;
   const uint64_t bound = lp_group_bound(sh, best, k);
   for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const uint64_t key = sh.cand[i];
+    const uint64_t key = get(i);
     if (key != 0 && key >= bound) sh.kept[atomicAdd(&sh.kept_count, 1)] = key;
   }
   if (threadIdx.x < kLpMaxTop) sh.best[threadIdx.x] = 0;
@@ -275,7 +283,18 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
   uint64_t bound = 0;
   float bound_x = -3.402823466e38f;  // every entry but -inf
   if (tid == 0) sh.count = 0;
+  // The targets' logits, on their way while the row is read (more than
+  // kLpThreads of them: the others at the end).
+  auto fetch_target = [&](int i) {
+    const int64_t id = p.targets[row * p.n_targets + i];
+    const int is = id < 0 ? -1 : id >= p.vocab;  // -1: no token, 1: past the vocabulary
+    sh.target_is[tid] = is;
+    if (is == 0) sh.target_x[tid] = Elem<T>::to(x[id]);
+  };
+  if (part == 0 && tid < p.n_targets) fetch_target(tid);
   __syncthreads();
+  // Says that this CTA runs: its shared memory may be written once all have.
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   auto id_of = [&](int slot, int bit) { return (slot + bit / VEC * kLpThreads) * VEC - skew + bit % VEC; };
   // Entries at or above the bound go to the buffer.
   auto collect = [&](const Batch& b, const float (&top)[kLpUnroll], int slot) {
@@ -331,8 +350,10 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       if (bm >= bound_x) collect(b, top, base + tid);
       // After 2, 4, 8 .. batches the bound rises with the maxima so far (their
       // ids are not kept: the key of any entry with that value will do), so
-      // that each doubling of what has been read adds about k candidates.
-      if (++batches > 1 && (batches & (batches - 1)) == 0) {
+      // that each doubling of what has been read adds about k candidates.  Not
+      // where less than half as much is left.
+      if (++batches > 1 && (batches & (batches - 1)) == 0 &&
+          ((end - base) / (kLpThreads * kLpUnroll) - 1) * 2 >= batches) {
         const uint64_t higher = lp_group_bound(sh, st.m > -INFINITY ? lp_key(st.m, 0xffffffffu - tid) : 0, k);
         if (higher != 0 && (higher | 0xffffffffu) > (bound | 0xffffffffu)) {
           bound = higher & ~0xffffffffull;
@@ -405,40 +426,47 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       }
       __syncthreads();
     }
-    lp_select(sh, sh.count, k);
   }
-  __syncthreads();
-
-  if (p.splits > 1) {
-    cluster_sync_all();  // every CTA's total and alternatives are in place
-    if (part == 0) {
-      if (tid == 0) {
-        LpStats t = sh.total;
-        for (int r = 1; r < p.splits; ++r) {
-          const uint32_t at = mapa_shared(smem_u32(&sh.total), r);
-          LpStats o;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(at));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.s) : "r"(at + 4));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.u) : "r"(at + 8));
-          t = lp_join(t, o, c);
-        }
-        sh.total = t;
-      }
-      if (k > 0) {
-        for (int i = tid; i < p.splits * k; i += kLpThreads) {
-          const int r = i / k;
-          const uint32_t at = mapa_shared(smem_u32(&sh.best[i - r * k]), r);
-          uint64_t key;
-          asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(at));
-          sh.cand[i] = key;
-        }
-        __syncthreads();
-        lp_select(sh, p.splits * k, k);
-      }
-      __syncthreads();
+  int found = sh.count;
+  if (p.splits == 1) {
+    if (k > 0) lp_select(sh, found, k, [&](int i) { return sh.cand[i]; });
+    __syncthreads();
+  } else {
+    // More candidates than the inbox holds: the k largest of them.
+    const uint64_t* send = sh.cand;
+    if (k > 0 && found > kLpInbox) {
+      lp_select(sh, found, k, [&](int i) { return sh.cand[i]; });
+      send = sh.best;
+      found = k;
     }
-    cluster_sync_all();  // no CTA leaves while its shared memory is read
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA runs
+    if (k > 0)
+      for (int i = tid; i < found; i += kLpThreads)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&sh.inbox[part * kLpInbox + i]), 0)),
+                     "l"(send[i])
+                     : "memory");
+    if (tid == 0) {
+      const uint32_t at = mapa_shared(smem_u32(&sh.part[part]), 0);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(st.m) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(st.s) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(st.u) : "memory");
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&sh.part_count[part]), 0)),
+                   "r"(k > 0 ? found : 0)
+                   : "memory");
+    }
+    __syncwarp();
+    cluster_sync_all();  // all has arrived
     if (part != 0) return;
+    if (tid < 32) {
+      LpStats t = tid < p.splits ? sh.part[tid] : LpStats{-INFINITY, 0.0f, 0.0f};
+      t = lp_join_lanes(t, c, kLpMaxSplits);
+      if (tid == 0) sh.total = t;
+    }
+    if (k > 0)
+      lp_select(sh, p.splits * kLpInbox, k, [&](int i) -> uint64_t {
+        return i % kLpInbox < sh.part_count[i / kLpInbox] ? sh.inbox[i] : 0;
+      });
+    __syncthreads();
   }
 
   const LpStats t = sh.total;
@@ -455,11 +483,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
     return (v - t.m) * p.inv_temperature - log_s;
   };
   for (int i = tid; i < p.n_targets; i += kLpThreads) {
-    const int64_t id = p.targets[row * p.n_targets + i];
-    float r = 0.0f;  // a negative id: no token
-    if (id >= p.vocab) r = __int_as_float(0x7fffffff);
-    else if (id >= 0) r = logp(Elem<T>::to(x[id]));
-    p.logprobs[row * p.n_targets + i] = r;
+    if (i >= kLpThreads) fetch_target(i);
+    const int is = sh.target_is[tid];
+    p.logprobs[row * p.n_targets + i] = is < 0 ? 0.0f : is ? __int_as_float(0x7fffffff) : logp(sh.target_x[tid]);
   }
   for (int i = tid; i < k; i += kLpThreads) {
     const uint64_t key = t.s != t.s ? 0 : sh.best[i];
