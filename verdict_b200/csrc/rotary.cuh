@@ -41,7 +41,7 @@ struct RotaryParams {
 
 constexpr int kRotaryTokens = 4;
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryUnroll = 4;  // units whose loads a thread has in flight
+constexpr int kRotaryUnroll = 2;  // units whose loads a thread has in flight
 
 __device__ __forceinline__ float2 rotary_cos_sin(int64_t pos, uint64_t turns) {
   // The top 32 bits of the fraction as a signed number: (-1/2, 1/2] turn.
@@ -56,7 +56,7 @@ __device__ __forceinline__ float2 rotary_cos_sin(int64_t pos, uint64_t turns) {
 // halves are multiples of eight, pointers 16-byte aligned); else a pair or an
 // element at a time.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, sizeof(T) == 2 ? 5 : 1) rotary_kernel(RotaryParams p) {
   extern __shared__ float2 cs[];  // [kRotaryTokens][rotary_dim / 2]
   const int half = p.rotary_dim >> 1;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRotaryTokens;
