@@ -205,6 +205,10 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
   if (s.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // The set-up above ran under the tail of the kernel before this one; global
+  // memory is touched only when that one is done.
+  pdl_trigger_next();
+  pdl_wait_prior();
 
   float acc[COLS];
   if (warp == 0) {
@@ -469,6 +473,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
   cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger_next();  // as in the other kernel
+  pdl_wait_prior();
 
   const int num_m = (s.M + 2 * BM - 1) / (2 * BM);
   const int num_n = (s.N + BN - 1) / BN;

@@ -59,10 +59,13 @@ int sm_count() {
 
 void launched() { cuda_check(cudaGetLastError(), "kernel launch"); }
 
+// cluster = 0: the kernel's own cluster size.  programmatic: the kernel may be
+// set up while the one before it in the stream still runs (it waits for that
+// one itself).
 template <class K, class... Args>
-void launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
-                    const Args&... args) {
-  if (cluster == 1) {
+void launch(K kernel, dim3 grid, int threads, size_t smem, int cluster, bool programmatic, cudaStream_t stream,
+            const Args&... args) {
+  if (cluster == 1 && !programmatic) {
     kernel<<<grid, threads, smem, stream>>>(args...);
     return launched();
   }
@@ -71,13 +74,21 @@ void launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, 
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  unsigned n = 0;
+  if (cluster > 0) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (programmatic) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
   cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), "kernel launch");
 }
 
@@ -157,9 +168,9 @@ void launch_f8_rows(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8
   s.splits = plan.splits;
   s.stages = plan.stages;
   const int n_tiles = (s.N + 127) / 128, m_tiles = (s.M + BN - 1) / BN;
-  launch_cluster(fp8_gemm_rows_kernel<BN, O>, dim3(n_tiles * s.splits, m_tiles), Cfg::THREADS,
-                 Cfg::smem_bytes(s.stages, s.splits), s.splits, stream, f8_map(w, s.N, s.K, ld_w, 128),
-                 f8_map(a, s.M, s.K, ld_a, BN), s, status);
+  launch(fp8_gemm_rows_kernel<BN, O>, dim3(n_tiles * s.splits, m_tiles), Cfg::THREADS,
+         Cfg::smem_bytes(s.stages, s.splits), s.splits, true, stream, f8_map(w, s.N, s.K, ld_w, 128),
+         f8_map(a, s.M, s.K, ld_a, BN), s, status);
 }
 
 // Row-major outputs [rows, cols] with row stride ld, boxes of 32 rows x 128
@@ -193,10 +204,9 @@ void launch_f8_pair(const void* a, int64_t ld_a, const void* w, int64_t ld_w, co
   if (attr.numRegs != Cfg::LAUNCH_REGS) fail(VD_ECUDA, "fp8_gemm_pair_kernel was built with another register count");
   const int tiles = ((s.M + 255) / 256) * ((s.N + 255) / 256);
   const int grid = 2 * std::min(tiles, sm_count() / 2);
-  kernel<<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(
-      f8_map(a, s.M, s.K, ld_a, 128), f8_map(w, s.N, s.K, ld_w, 128),
-      s.out_aligned ? out_map(s.out, s.M, s.N, s.ld_out, dtype) : CUtensorMap{}, s, status);
-  launched();
+  launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM_BYTES, 0, true, stream, f8_map(a, s.M, s.K, ld_a, 128),
+         f8_map(w, s.N, s.K, ld_w, 128), s.out_aligned ? out_map(s.out, s.M, s.N, s.ld_out, dtype) : CUtensorMap{}, s,
+         status);
 }
 
 }  // namespace
@@ -544,8 +554,8 @@ extern "C" VD_API int vdk_token_logprobs(const void* logits, int64_t ld, int64_t
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     by_type(dtype, [&](auto tag) {
       using T = decltype(tag);
-      launch_cluster(token_logprobs_kernel<T>, dim3(static_cast<unsigned>(rows * p.splits)), kLpThreads,
-                     sizeof(LpShared), p.splits, s, p);
+      launch(token_logprobs_kernel<T>, dim3(static_cast<unsigned>(rows * p.splits)), kLpThreads, sizeof(LpShared),
+             p.splits, false, s, p);
     });
   });
 }
