@@ -55,18 +55,19 @@ template <bool FULL, class T>
 __device__ __forceinline__ void columns4(const T* p, int n, float (&v)[4]) {
   Chunk4<T> c;
   if (FULL) c.load(p);
-  else c.load_part(p, n);
+  else c.load_gap(p, n);
   c.get(v);
 }
 
 // FULL: every thread has NV whole, aligned chunks (cols = 4 NV blockDim.x);
-// otherwise element by element.
+// otherwise element by element, a thread's four 32 columns apart.
 template <class TY, class TH, int NV, bool FULL>
 __global__ void block_norm_kernel(BlockNormParams p) {
   __shared__ float slots[2][32];
   const int64_t row = blockIdx.x;
   const int step = blockDim.x * 4;
-  const int col0 = threadIdx.x * 4;
+  const int col0 = FULL ? threadIdx.x * 4 : (threadIdx.x >> 5) * 128 + (threadIdx.x & 31);
+  constexpr int GAP = FULL ? 1 : kGap;
   Chunk4<TY> yr[NV];
   Chunk4<TH> hr[NV];
 #pragma unroll
@@ -76,7 +77,7 @@ __global__ void block_norm_kernel(BlockNormParams p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (FULL) yr[i].load(y + i * step);
-      else yr[i].load_part(y + i * step, p.cols - col0 - i * step);
+      else yr[i].load_gap(y + i * step, p.cols - col0 - i * step);
     }
   }
   if (p.h) {
@@ -84,7 +85,7 @@ __global__ void block_norm_kernel(BlockNormParams p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (FULL) hr[i].load(h + i * step);
-      else hr[i].load_part(h + i * step, p.cols - col0 - i * step);
+      else hr[i].load_gap(h + i * step, p.cols - col0 - i * step);
     }
   }
   const float inv_cols = 1.0f / static_cast<float>(p.cols);
@@ -160,12 +161,12 @@ __global__ void block_norm_kernel(BlockNormParams p) {
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (FULL || col0 + i * step + j < p.cols) m = max(m, magnitude_bits(u[i][j]));
+        if (FULL || col0 + i * step + j * GAP < p.cols) m = max(m, magnitude_bits(u[i][j]));
       m = __reduce_max_sync(0xffffffffu, m);
       if (lane == i) mine = m;
     }
     const F8Scale s = f8_scale(mine);
-    const int block0 = col0 / kF8Block;
+    const int block0 = col0 / kF8Block;  // the warp's first
     if (lane < NV && (block0 + lane * (step / kF8Block)) * kF8Block < p.cols)
       p.z_scale[row * p.ld_scale + block0 + lane * (step / kF8Block)] = s.scale;
     uint8_t* o = static_cast<uint8_t*>(p.z) + at;
@@ -178,7 +179,7 @@ __global__ void block_norm_kernel(BlockNormParams p) {
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (j < n) o[i * step + j] = static_cast<uint8_t>(q >> (8 * j));
+          if (j * GAP < n) o[i * step + j * GAP] = static_cast<uint8_t>(q >> (8 * j));
       }
     }
     return;

@@ -606,23 +606,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
       }
       if (!ok) break;
       if (s.bias) {
+        if (col0 + 128 <= s.N && (reinterpret_cast<uintptr_t>(s.bias) & 15) == 0) {
+          const float4* b = reinterpret_cast<const float4*>(s.bias + col0);
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          const int col = col0 + 2 * j;
-          if (col < s.N) acc[j].x += __ldg(s.bias + col);
-          if (col + 1 < s.N) acc[j].y += __ldg(s.bias + col + 1);
-        }
-      }
-      if (!s.out_aligned) {  // rows of out that TMA cannot address
-        if (row < s.M) {
-          O* o = static_cast<O*>(s.out) + row * s.ld_out + col0;
+          for (int j = 0; j < 32; ++j) {
+            const float4 v = __ldg(b + j);
+            acc[2 * j] = __fadd2_rn(acc[2 * j], make_float2(v.x, v.y));
+            acc[2 * j + 1] = __fadd2_rn(acc[2 * j + 1], make_float2(v.z, v.w));
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
-            if (col0 + 2 * j < s.N) o[2 * j] = Elem<O>::from(acc[j].x);
-            if (col0 + 2 * j + 1 < s.N) o[2 * j + 1] = Elem<O>::from(acc[j].y);
+            const int col = col0 + 2 * j;
+            if (col < s.N) acc[j].x += __ldg(s.bias + col);
+            if (col + 1 < s.N) acc[j].y += __ldg(s.bias + col + 1);
           }
         }
-        continue;
       }
 #pragma unroll
       for (int c = 0; c < 128 / CHUNK; ++c) {
@@ -643,12 +642,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
           }
           *reinterpret_cast<uint4*>(stage_out + lane * 128 + ((q ^ (lane & 7)) << 4)) = w;
         }
-        fence_proxy_async_smem_gemm();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&tmC, stage_out, x, row0);
-          bulk_commit();
+        if (s.out_aligned) {
+          fence_proxy_async_smem_gemm();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, stage_out, x, row0);
+            bulk_commit();
+          }
+          continue;
         }
+        // Rows of out that TMA cannot address: row by row, lanes along columns.
+        __syncwarp();
+        constexpr int EL = 4 / sizeof(O);  // outputs in a lane's four bytes
+        const int left = s.N - x - lane * EL, rows = min(32, s.M - row0);
+        O* o = static_cast<O*>(s.out) + row0 * s.ld_out + x + lane * EL;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r, o += s.ld_out) {
+          const uint32_t v =
+              *reinterpret_cast<const uint32_t*>(stage_out + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          const O* e = reinterpret_cast<const O*>(&v);
+#pragma unroll
+          for (int k = 0; k < EL; ++k)
+            if (k < left) o[k] = e[k];
+        }
+        __syncwarp();
       }
     }
     if (lane == 0) bulk_wait_all();

@@ -52,12 +52,17 @@ template <class T, int GATE, bool WHOLE>
 __global__ void __launch_bounds__(kQuantThreads, WHOLE && sizeof(T) == 2 ? 6 : 1) quantize_rows_kernel(QuantizeParams p) {
   const int lane16 = threadIdx.x & 15;
   const uint32_t first = blockIdx.x * (kQuantUnroll * kQuantThreads / 16) + (threadIdx.x >> 4);
-  Chunk8<T> xr[kQuantUnroll], gr[kQuantUnroll];
+  // A lane's eight columns of a block: neighbours, or 16 apart so that the
+  // lanes' single accesses are contiguous.
+  const int lane_col = WHOLE ? lane16 * 8 : lane16;
+  constexpr int GAP = WHOLE ? 1 : 16;
+  using Chunk = typename std::conditional<WHOLE, Chunk8<T>, T[8]>::type;
+  Chunk xr[kQuantUnroll], gr[kQuantUnroll];
 #pragma unroll
   for (int u = 0; u < kQuantUnroll; ++u) {
     const uint32_t id = first + u * (kQuantThreads / 16);
     const uint32_t row = p.per_row(id);
-    const int col = static_cast<int>(id - row * p.col_blocks) * kF8Block + lane16 * 8;
+    const int col = static_cast<int>(id - row * p.col_blocks) * kF8Block + lane_col;
     const int n = id < p.blocks ? p.cols - col : 0;
     const T* x = static_cast<const T*>(p.x) + row * p.ld_x + col;
     const T* g = GATE != kGateNone ? static_cast<const T*>(p.gate) + row * p.ld_gate + col : nullptr;
@@ -69,8 +74,11 @@ __global__ void __launch_bounds__(kQuantThreads, WHOLE && sizeof(T) == 2 ? 6 : 1
         if (GATE != kGateNone) gr[u].load(g);
       }
     } else {
-      xr[u].load_part(x, n);
-      if (GATE != kGateNone) gr[u].load_part(g, n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xr[u][j] = j * GAP < n ? x[j * GAP] : Elem<T>::from(0.0f);
+        if (GATE != kGateNone) gr[u][j] = j * GAP < n ? g[j * GAP] : Elem<T>::from(0.0f);
+      }
     }
   }
 #pragma unroll
@@ -78,26 +86,35 @@ __global__ void __launch_bounds__(kQuantThreads, WHOLE && sizeof(T) == 2 ? 6 : 1
     const uint32_t id = first + u * (kQuantThreads / 16);
     const uint32_t row = p.per_row(id);
     const uint32_t kb = id - row * p.col_blocks;
-    const int col = static_cast<int>(kb) * kF8Block + lane16 * 8;
-    float v[8];
-    xr[u].get(v);
-    if (GATE != kGateNone) {
-      float g[8];
-      gr[u].get(g);
+    const int col = static_cast<int>(kb) * kF8Block + lane_col;
+    float v[8], g[8];
+    if constexpr (WHOLE) {
+      xr[u].get(v);
+      if (GATE != kGateNone) gr[u].get(g);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= gate_act<GATE>(g[j], p.act);
+      for (int j = 0; j < 8; ++j) {
+        v[j] = Elem<T>::to(xr[u][j]);
+        if (GATE != kGateNone) g[j] = Elem<T>::to(gr[u][j]);
+      }
     }
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, magnitude_bits(v[j]));
+    for (int j = 0; j < 8; ++j) {
+      if (GATE != kGateNone) v[j] *= gate_act<GATE>(g[j], p.act);
+      m = max(m, magnitude_bits(v[j]));
+    }
     const F8Scale s = f8_scale(max16(m));
     if (id < p.blocks) {
       if (lane16 == 0) p.scale[row * p.ld_scale + kb] = s.scale;
       uint8_t* q = p.q + row * p.ld_q + col;
+      const uint2 w = f8_pack8(v, s.inv);
       if constexpr (WHOLE) {
-        if (col < p.cols) *reinterpret_cast<uint2*>(q) = f8_pack8(v, s.inv);
+        if (col < p.cols) *reinterpret_cast<uint2*>(q) = w;
       } else {
-        f8_store(q, f8_pack8(v, s.inv), p.cols - col, false);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j * GAP < p.cols - col) q[j * GAP] = static_cast<uint8_t>((j < 4 ? w.x : w.y) >> ((j & 3) * 8));
       }
     }
   }
@@ -133,7 +150,7 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const T* __restric
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = row0 + i * 16;
-    if (row < rows && col < cols) f8_store(q + row * ld_q + col, f8_pack8(v[i], s.inv), cols - col, false);
+    if (row < rows && col < cols) f8_store(q + row * ld_q + col, f8_pack8(v[i], s.inv), cols - col);
   }
 }
 

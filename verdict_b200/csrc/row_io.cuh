@@ -84,6 +84,10 @@ struct Chunk8<float> {
   }
 };
 
+// Rows that vector accesses do not fit: a warp takes 128 columns, a lane
+// every 32nd of them.
+constexpr int kGap = 32;
+
 // Four elements: 8 bytes of a 16-bit type, 16 of fp32.  A warp's access is
 // contiguous in either, which eight fp32 elements a thread are not (two
 // accesses of every other 16 bytes: twice the shared L1 wavefronts).
@@ -95,13 +99,15 @@ struct Chunk4 {
     else r = make_uint2(0, 0);
   }
   __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const decltype(r)*>(p); }
-  __device__ __forceinline__ void load_part(const T* p, int n) {
+  // Elements kGap apart (a warp's accesses contiguous), those below n.
+  __device__ __forceinline__ void load_gap(const T* p, int n) {
+    constexpr int G = kGap;
     if constexpr (sizeof(T) == 4) {
-      r = make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+      r = make_float4(n > 0 ? p[0] : 0.f, n > G ? p[G] : 0.f, n > 2 * G ? p[2 * G] : 0.f, n > 3 * G ? p[3 * G] : 0.f);
     } else {
       const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-      r.x = (n > 0 ? s[0] : 0u) | ((n > 1 ? s[1] : 0u) << 16);
-      r.y = (n > 2 ? s[2] : 0u) | ((n > 3 ? s[3] : 0u) << 16);
+      r.x = (n > 0 ? s[0] : 0u) | ((n > G ? s[G] : 0u) << 16);
+      r.y = (n > 2 * G ? s[2 * G] : 0u) | ((n > 3 * G ? s[3 * G] : 0u) << 16);
     }
   }
   __device__ __forceinline__ void get(float (&v)[4]) const {
@@ -122,7 +128,7 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int n) {
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j < n) p[j] = Elem<T>::from(v[j]);
+      if (j * kGap < n) p[j * kGap] = Elem<T>::from(v[j]);
   }
 }
 
@@ -171,12 +177,7 @@ __device__ __forceinline__ uint2 f8_pack8(const float (&v)[8], float inv) {
                     f8_pack2(v[4], v[5], inv) | (f8_pack2(v[6], v[7], inv) << 16));
 }
 
-// n < 8 or an unaligned row: byte stores.
-__device__ __forceinline__ void f8_store(uint8_t* p, uint2 q, int n, bool aligned) {
-  if (aligned && n >= 8) {
-    *reinterpret_cast<uint2*>(p) = q;
-    return;
-  }
+__device__ __forceinline__ void f8_store(uint8_t* p, uint2 q, int n) {
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (j < n) p[j] = static_cast<uint8_t>((j < 4 ? q.x : q.y) >> ((j & 3) * 8));
