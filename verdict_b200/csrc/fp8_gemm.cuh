@@ -120,8 +120,12 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
 // token's column through distributed shared memory, and that one adds them in
 // rank order, so the result does not depend on who came first.
 //
-// A drain thread owns a weight row.  The scales a[token] * w of 16 k-blocks at
-// a time lie in shared memory and are read four tokens at once.
+// A drain thread owns a weight row.  The scales a[token] * w of 8 or 16
+// k-blocks at a time lie in shared memory and are read four tokens at once.
+//
+// bf16, device time: 1 x 6144 x 4096 6.7 us (floor 3.8: the weights' 25 MB),
+// 16 x 24576 x 4096 20.5 us (4.9 TB/s), 37 x 4096 x 12288 15.8 us (floor 7.8;
+// while it streams 5.5 TB/s, the rest is the first loads' latency and the join).
 // ---------------------------------------------------------------------------
 template <int BN>
 struct F8RowsConfig {
@@ -388,6 +392,17 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
 // registers while the next k-block's MMAs fill the other.  The grid is
 // persistent, one pair per two SMs; outputs leave through shared memory and
 // TMA stores while the next tile's MMAs run.
+//
+// 8192 x 24576 x 4096 bf16: 890-910 us, 1.83 PFLOP/s back to back, under the
+// power cap (1000 W, 1515 MHz); 760 us, 2.17 PFLOP/s, in short bursts.  515 x
+// 6144 x 4096: 24 us.  A k-block takes about 890 cycles, 512 of them MMAs: two
+// accumulators are all that TMEM holds at this width, and the way from a
+// finished accumulator to its reuse (two 64-column loads with the first half's
+// FMAs between them, 325 cycles, then the hand-back to the leader and the MMAs'
+// own 750 cycles of latency) is longer than one k-block.  Tried, slower: 16
+// drain warps of 64 columns (1030 cycles), 32-column loads in two buffers
+// (950), scales four k-blocks ahead (920), MMAs of N = 128 with four
+// accumulators (1120: A is read twice).
 // ---------------------------------------------------------------------------
 struct F8PairConfig {
   static constexpr int BM = 128;  // rows per CTA

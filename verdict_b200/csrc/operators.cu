@@ -318,7 +318,7 @@ extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a
       const int pair_tiles = ((s.M + 255) / 256) * ((s.N + 255) / 256);
       const int pair_steps = (pair_tiles + pairs - 1) / pairs * ((s.K + 127) / 128);
       const F8RowsPlan plan = plan_f8_rows<128, O>(s);
-      if (plan.steps * 1.1 + 4 < pair_steps) launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, plan, status, st);
+      if (plan.steps * 1.1 + 4 < pair_steps && (M + 127) / 128 <= 65535) launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, plan, status, st);
       else launch_f8_pair<O>(a, ld_a, w, ld_w, s, out_dtype, status, st);
     });
   });

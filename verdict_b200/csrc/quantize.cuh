@@ -9,7 +9,10 @@
 // Bound by memory: one read of x (and gate), one write of a byte per element.
 // 16 lanes hold a block (8 elements each, one 16-byte load for 16-bit types),
 // so its maximum is four shuffles; each thread takes kQuantUnroll blocks,
-// whose loads are all issued before the first is used.
+// whose loads are all issued before the first is used.  Two blocks a thread
+// and six CTAs on an SM (40 registers) beat four and three (145 -> 90 us).
+// Gated 8192 x 12288 fp16 with SiLU: 92 us, 5.5 TB/s, 0.84 of the measured
+// copy rate; ungated fp32 8192 x 5120: 34 us, 6.3 TB/s.
 #pragma once
 
 #include "gemm.cuh"

@@ -12,7 +12,11 @@
 //
 // Bound by memory: q and k are read and written once.  A CTA takes
 // kRotaryTokens tokens: it forms their cosines and sines once, in shared
-// memory, and every head of those tokens reads them there.
+// memory, and every head of those tokens reads them there.  One unit in flight
+// a thread left loads exposed (79 us below), four cost occupancy (71).
+// 16384 tokens of 16 + 4 heads of 256, 64 columns rotated, fp16: 65 us, 5.2
+// TB/s, 0.79 of the measured copy rate; 12288 of 32 + 8 heads of 128, fp32: 82
+// us, 6.1 TB/s.
 #pragma once
 
 #include "row_io.cuh"

@@ -18,8 +18,15 @@
 // buffer; it is then read again for a bound found by radix selection, at most
 // eight more times.
 //
-// Few rows: a cluster of up to eight CTAs shares a row and joins through
-// distributed shared memory.
+// Few rows: a cluster of up to eight CTAs shares a row; each pushes its sums
+// and candidates to the first through distributed shared memory.
+//
+// 1024 x 256000 bf16, 8 alternatives: 136 us, 3.9 TB/s, 0.59 of the measured
+// copy rate.  The logits alone are 80 us; the rest is arithmetic (issue slots
+// 61 %, special-function unit 49 %: an exp2 an entry) and the 1.7 waves that
+// 1024 rows make of 592 resident CTAs.  Four loads a thread and four CTAs on an
+// SM beat two and five or six (165, 183 us) and eight and three (158).  One row
+// of 152064: 12 us, latency.
 #pragma once
 
 #include <type_traits>

@@ -102,7 +102,8 @@ def fp8_linear(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """a @ w.T + bias: a e4m3 [M, K] with scales [M, ceil(K / 128)], w e4m3 [N, K] with scales
     [ceil(N / 128), ceil(K / 128)]; out [M, N] of out_dtype.  Rows of a and w start on 16-byte boundaries (as the
-    casts lay them out).  The first call on a device waits for it once (the word that check_status reads)."""
+    casts lay them out).  The first call on a device makes the word that check_status reads and waits for it once: make
+    that call before any stream capture."""
     code = _CODES.get(out_dtype)
     if code is None:
         raise ValueError(f"out_dtype must be one of {[str(d) for d in _CODES]}")
