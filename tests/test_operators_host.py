@@ -174,3 +174,12 @@ def test_c_entries_check_before_they_launch():
     # A null error buffer is allowed.
     assert _abi.load().vdk_token_logprobs(FAKE, 10, 2, 20, 0, 1.0, None, 0, 0, None, None, None, None, None, None, None,
                                           0) == E
+
+
+def test_rotary_outputs_that_overlap_are_refused():
+    H = _abi.VdkRotaryHeads
+    # (token stride, head stride) of 3 tokens x 2 heads of 64
+    for token, head in ((64, 64), (0, 64), (100, 64), (64, 100), (32, 128)):
+        rc, msg = call("vdk_rotary", H(FAKE, FAKE, 128, 64, token, head, 2), None, 3, 64, 64, 0, 0, 0, None, 0, 0, FAKE,
+                       1.0)
+        assert rc == _abi.VD_EINVAL and "overlap" in msg, (token, head, msg)

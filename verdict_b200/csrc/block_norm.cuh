@@ -11,10 +11,11 @@
 // row; a thread keeps NV chunks of four columns in registers through both
 // norms, so nothing is read twice.  Four columns make every access of a warp
 // contiguous, the gains' (fp32, read by every row) among them: eight kept the
-// L1 L1 busy 74 % of the time.
+// L1 busy 74 % of the time.
 // 16384 x 4096, y bf16, residual fp32, 8-bit z: 134 us, 5.5 TB/s, 0.84 of the
 // measured copy rate; what is left is the two reductions' latency at four CTAs
-// on an SM (five at 48 registers were no faster).#pragma once
+// on an SM (five at 48 registers were no faster).
+#pragma once
 
 #include "row_io.cuh"
 

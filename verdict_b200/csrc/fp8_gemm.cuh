@@ -53,6 +53,14 @@ __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile
   }
 }
 
+// After a wait ran out: the last phase that a ring's barriers were armed for,
+// slots before `at` in the pass with parity `phase`, the others in the one
+// before (true at once where that never was).  Lets the copies and MMAs that
+// are under way land before the CTA gives up its memory.
+__device__ __forceinline__ void f8_settle(uint64_t* bars, int n, int at, uint32_t phase) {
+  for (int i = 0; i < n; ++i) mbar_wait_own(&bars[i], i < at ? phase : phase ^ 1, VD_WAIT_TIMEOUT_NS / 8);
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, e4m3 inputs, fp32 accumulate.
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -229,10 +237,13 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
         if (++stage == stages) stage = 0, phase ^= 1;
       }
       // Every load has landed and been consumed before the CTA may exit.
+      const int at = stage;
+      const uint32_t at_phase = phase;
       for (int i = 0; i < stages && ok; ++i) {
         ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
         if (++stage == stages) stage = 0, phase ^= 1;
       }
+      if (!ok) f8_settle(full, stages, at, at_phase);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -243,7 +254,10 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
       bool ok = f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty) &&
                 f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!ok) {
+        f8_settle(acc_full, BUFS, buf, buf_phase);
+        break;
+      }
       tc_fence_after();
       if (elect_one()) {
         // Descriptors hold addresses in units of 16 bytes; 32 bytes per step of K.
@@ -525,10 +539,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
           }
         }
         // Every stage this CTA filled has been consumed before the CTA may exit.
+        const int at = stage;
+        const uint32_t at_phase = phase;
         for (int i = 0; i < STAGES && ok; ++i) {
           ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
+        // The leader's barriers count both CTAs' loads; the other CTA meets it
+        // at the cluster barrier below.
+        if (!ok && leader) f8_settle(full, STAGES, at, at_phase);
       }
     } else if (warp == 1) {
       // The whole warp waits and one elected lane issues, so that addresses and
@@ -544,7 +563,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
             ok = f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull) &&
                  f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            if (!ok) {
+              f8_settle(acc_full, 2, buf, buf_phase);
+              break;
+            }
             tc_fence_after();
             if (elect_one()) {
               // Descriptors hold addresses in units of 16 bytes; 32 bytes per step of K.

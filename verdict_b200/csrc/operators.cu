@@ -482,7 +482,11 @@ extern "C" VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_hea
       need(v->heads >= 1 && v->heads <= 65536, "heads must be from 1 to 65536");
       need(tokens == 0 || (v->in && v->out), "null buffer");
       need(v->in_token >= 0 && v->in_head >= 0 && v->out_token >= 0 && v->out_head >= 0, "negative stride");
-      need(v->heads == 1 || v->out_head >= head_dim, "output heads overlap");
+      // Output rows of head_dim lie apart: heads within a token, or tokens within a head.
+      const int64_t hs = v->out_head, ts = v->out_token;
+      need((v->heads == 1 || hs >= head_dim) && (tokens <= 1 || ts >= head_dim) &&
+               (v->heads == 1 || tokens <= 1 || ts / v->heads >= hs || hs / tokens >= ts),
+           "output heads overlap");
       r = {v->in, v->out, v->in_token, v->in_head, v->out_token, v->out_head, v->heads};
       for (const int64_t st : {v->in_token, v->in_head, v->out_token, v->out_head}) vec = vec && st * es % 16 == 0;
       vec = vec && aligned16(v->in) && aligned16(v->out);

@@ -138,6 +138,11 @@ int64_t integer(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw Raised();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised();
+  return v != 0;
+}
 double real(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw Raised();
@@ -244,7 +249,7 @@ PyObject* block_norm(PyObject* const* p) {
   const Tensor *y = optional(p[0], "y"), *h = optional(p[1], "residual"), *post = optional(p[2], "post_gain"),
                *gate = optional(p[3], "gate"), *pre = optional(p[6], "pre_gain");
   const double residual_scale = real(p[4]), block_scale = real(p[5]), eps = real(p[7]);
-  const bool plus_one = PyObject_IsTrue(p[8]), in_place = PyObject_IsTrue(p[10]);
+  const bool plus_one = truth(p[8]), in_place = truth(p[10]);
   int out_code = static_cast<int>(integer(p[9]));
   if (!y && !h) refuse("need y or a residual");
   const Tensor& x = y ? *y : *h;
@@ -329,7 +334,7 @@ PyObject* rotary(PyObject* const* p) {
   if (turns.device() != x.device())
     refuse("the plan is on " + turns.device().str() + ", q and k on " + x.device().str());
   const int64_t head_dim = integer(p[4]), rotary_dim = integer(p[5]);
-  const bool interleaved = PyObject_IsTrue(p[6]), inverse = PyObject_IsTrue(p[8]);
+  const bool interleaved = truth(p[6]), inverse = truth(p[8]);
   const float factor = static_cast<float>(real(p[7]));
   Tensor outs[2];
   vdk_rotary_heads heads[2];
@@ -401,9 +406,10 @@ PyObject* token_logprobs(PyObject* const* p) {  // logits, ids, top, temperature
     top_ids = empty({rows, top}, ScalarType::Int, x);
     top_lp = empty({rows, top}, ScalarType::Float, x);
   }
+  const float temperature = static_cast<float>(real(p[3]));
   if (rows)
     run(x, [&](void* s, char* e, size_t len) {
-      return vdk_token_logprobs(ptr(x), ld(x), rows, vocab, code(type_of(x)), static_cast<float>(real(p[3])),
+      return vdk_token_logprobs(ptr(x), ld(x), rows, vocab, code(type_of(x)), temperature,
                                 n ? static_cast<const int64_t*>(ptr(ids)) : nullptr, n, static_cast<int>(top),
                                 n ? static_cast<float*>(ptr(lp)) : nullptr, static_cast<float*>(ptr(entropy)),
                                 static_cast<float*>(ptr(lse)), top ? static_cast<int32_t*>(ptr(top_ids)) : nullptr,
