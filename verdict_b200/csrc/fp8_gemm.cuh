@@ -416,7 +416,8 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
 // own 750 cycles of latency) is longer than one k-block.  Tried, slower: 16
 // drain warps of 64 columns (1030 cycles), 32-column loads in two buffers
 // (950), scales four k-blocks ahead (920), MMAs of N = 128 with four
-// accumulators (1120: A is read twice).
+// accumulators (1120: A is read twice), 192-column tiles whose 96 columns a
+// warp loads at once and hands back before any FMA (1057 us).
 // ---------------------------------------------------------------------------
 struct F8PairConfig {
   static constexpr int BM = 128;  // rows per CTA
