@@ -612,3 +612,43 @@ def test_refusals():
         with pytest.raises(_abi.VdError):
             f()
             pytest.fail(f"case {i} was accepted")
+
+
+# ---------------------------------------------------------------------------
+# Rows far apart
+# ---------------------------------------------------------------------------
+def test_offsets_past_32_bits():
+    """Rows 2^30 elements apart (the third starts past 2^31) give what the same rows give side by side."""
+    step = 1 << 30
+    buf = torch.empty(2 * step + 8192, dtype=torch.bfloat16, device="cuda")
+
+    def far(t):
+        v = buf.as_strided(t.shape, (step, 1))
+        v.copy_(t)
+        return v
+
+    g = gen(21)
+    x = randn(g, 3, 2056, dtype=torch.bfloat16, scale=2.0)
+    gain = 1 + randn(g, 2056, scale=0.1)
+    q, s = ops.quantize_fp8(x)
+    qf, sf = ops.quantize_fp8(far(x))
+    assert torch.equal(q.float(), qf.float()) and torch.equal(s, sf)
+    r, rf = ops.block_norm(x, x, post_gain=gain, pre_gain=gain), ops.block_norm(far(x), x, post_gain=gain, pre_gain=gain)
+    assert torch.equal(r.out, rf.out) and torch.equal(r.residual, rf.residual)
+    ids = torch.tensor([[5, 2055]] * 3, device="cuda")
+    lp, lpf = ops.token_logprobs(x, ids, top=7), ops.token_logprobs(far(x), ids, top=7)
+    assert all(torch.equal(a, b) for a, b in zip(lp, lpf))
+    w, sw = operand(g, 2056, 2056, 128)
+    out = ops.fp8_linear(q, s, w, sw)
+    assert torch.equal(ops.fp8_linear(q, s, w, sw, out=buf.as_strided((3, 2056), (step, 1))), out)
+    a = buf.view(torch.uint8).as_strided((3, 2056), (step, 1))
+    a.copy_(q.view(torch.uint8) if q.is_contiguous() else q.contiguous().view(torch.uint8))
+    assert torch.equal(ops.fp8_linear(a.view(F8), s, w, sw), out)
+    plan = ops.RotaryPlan(128)
+    heads = x[:, :1024].unflatten(1, (8, 128))
+    pos = torch.tensor([3, 70000, 1], device="cuda")
+    want, _ = ops.rotary(heads, None, pos, plan)
+    v = buf.as_strided((3, 8, 128), (step, 128, 1))
+    v.copy_(heads)
+    got, _ = ops.rotary(v, None, pos, plan, q_out=v)
+    assert torch.equal(got, want)
