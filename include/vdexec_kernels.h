@@ -153,6 +153,17 @@ VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int
                           char* err, size_t errlen);
 
 /*
+ * Failure-path tests only: the same with a limit of its own on every pipeline
+ * wait, and with each CTA's loads stopping after stall_after blocks of 128
+ * columns (-1: never).  Where they stop early, a wait runs out: the kernel
+ * ends, status has the wait's code and out is not to be used.
+ */
+VD_API int vdk_fp8_linear_stalled(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale, const void* w,
+                                  int64_t ld_w, const float* w_scale, int64_t ld_w_scale, int64_t M, int64_t N,
+                                  int64_t K, const float* bias, void* out, int64_t ld_out, int out_dtype, int* status,
+                                  int64_t wait_limit_us, int stall_after, void* stream, char* err, size_t errlen);
+
+/*
  * The step between two blocks of a decoder, one pass:
  *   u = rmsnorm(y) * post_gain, or y without post_gain;
  *   h_out = residual_scale * h + block_scale * gate * u;

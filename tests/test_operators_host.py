@@ -183,3 +183,12 @@ def test_rotary_outputs_that_overlap_are_refused():
         rc, msg = call("vdk_rotary", H(FAKE, FAKE, 128, 64, token, head, 2), None, 3, 64, 64, 0, 0, 0, None, 0, 0, FAKE,
                        1.0)
         assert rc == _abi.VD_EINVAL and "overlap" in msg, (token, head, msg)
+
+
+def test_limits_of_the_failure_path_entry():
+    # zero rows: nothing is launched, only the limits are looked at
+    args = (None, 128, None, 1, FAKE, 128, FAKE, 1, 0, 4, 128, None, None, 4, 0, None)
+    assert call("vdk_fp8_linear_stalled", *args, 1000, -1)[0] == _abi.VD_OK
+    for limit, stall in ((0, 0), (-1, 0), (2000001, 0), (1000, -2)):
+        rc, msg = call("vdk_fp8_linear_stalled", *args, limit, stall)
+        assert rc == _abi.VD_EINVAL and msg

@@ -29,12 +29,18 @@ struct F8Shape {
   int out_aligned;  // rows of out start on 16 bytes
   int splits;       // CTAs along K: the cluster's size
   int stages;       // of the shared-memory ring (fp8_gemm_rows_kernel)
+  // Failure-path tests: the limit of every barrier wait, and the k-blocks after
+  // which each CTA stops loading (-1: never), so that its other warps wait for a
+  // stage that nothing will fill.
+  uint64_t wait_ns = VD_WAIT_TIMEOUT_NS;
+  int stall_after = -1;
 };
 
 // mbar_wait with the clock read only after a run of polls: reading the global
 // timer takes longer than the k-block that most waits here are for.
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+__device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code,
+                                        uint64_t limit_ns) {
   uint64_t t0 = 0;
   while (true) {
 #pragma unroll 1
@@ -45,7 +51,7 @@ __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile
     const uint64_t t = globaltimer();
     if (t0 == 0) {
       t0 = t;
-    } else if (t - t0 > VD_WAIT_TIMEOUT_NS) {
+    } else if (t - t0 > limit_ns) {
       *abort_flag = 1;
       record_error(err, code);
       return false;
@@ -229,7 +235,8 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
       uint32_t phase = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
+        if (kb - kb0 == s.stall_after) break;
+        ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty, s.wait_ns);
         if (!ok) break;
         mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
         tma_load_2d(sW + stage * Cfg::W_BYTES, &tmW, &full[stage], kb * BK, n0);
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
       const int at = stage;
       const uint32_t at_phase = phase;
       for (int i = 0; i < stages && ok; ++i) {
-        ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
+        ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty, s.wait_ns);
         if (++stage == stages) stage = 0, phase ^= 1;
       }
       if (!ok) f8_settle(full, stages, at, at_phase);
@@ -251,11 +258,12 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
     uint32_t phase = 0, buf_phase = 0;
     const uint64_t w_desc0 = sw128_kmajor_desc(smem_u32(sW)), a_desc0 = sw128_kmajor_desc(smem_u32(sA));
     for (int kb = kb0; kb < kb1; ++kb) {
-      bool ok = f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty) &&
-                f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull);
+      bool ok = f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty, s.wait_ns) &&
+                f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull, s.wait_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         f8_settle(acc_full, BUFS, buf, buf_phase);
+        f8_settle(empty, stages, stage, phase);
         break;
       }
       tc_fence_after();
@@ -305,14 +313,16 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
     int buf = 0, chunk = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
-    for (int base = kb0; base < kb1 && ok; base += Cfg::SCALE_KB, ++chunk) {
-      // The chunk is in place; the other buffer's chunk has been used up.
+    for (int base = kb0; base < kb1; base += Cfg::SCALE_KB, ++chunk) {
+      // The chunk is in place; the other buffer's chunk has been used up.  A warp
+      // whose wait ran out keeps coming here: the others may still be at work, and
+      // this barrier counts on all of them.
       asm volatile("bar.sync 1, %0;" ::"n"(DRAIN) : "memory");
       const int stop = min(base + Cfg::SCALE_KB, kb1);
       if (stop < kb1) fetch(stop);
       const float* scales = sScale + (chunk & 1) * (Cfg::SCALE_KB * BN) + col0;
-      for (int kb = base; kb < stop; ++kb, scales += BN) {
-        ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull));
+      for (int kb = base; kb < stop && ok; ++kb, scales += BN) {
+        ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull, s.wait_ns));
         if (!ok) break;
         tc_fence_after();
         uint32_t r[COLS];
@@ -519,16 +529,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
         tma_prefetch_desc(&tmC);
-        int stage = 0;
+        int stage = 0, issued = 0;
         uint32_t phase = 0;
-        bool ok = true;
-        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        bool ok = true, stalled = false;
+        for (int tile = pair; tile < tiles && ok && !stalled; tile += pairs) {
           int m, n;
           tile_coords(tile, num_m, num_n, Cfg::GROUP_M, m, n);
           const int ya = m * 2 * BM + static_cast<int>(rank) * BM;
           const int yb = n * BN + static_cast<int>(rank) * (BN / 2);
           for (int kb = 0; kb < kblocks; ++kb) {
-            if (!f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty)) {
+            if (issued++ == s.stall_after) {
+              stalled = true;
+              break;
+            }
+            if (!f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty, s.wait_ns)) {
               ok = false;
               break;
             }
@@ -543,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
         const int at = stage;
         const uint32_t at_phase = phase;
         for (int i = 0; i < STAGES && ok; ++i) {
-          ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty);
+          ok = f8_wait(&empty[stage], phase ^ 1, abort_flag, err, kErrTimeoutEmpty, s.wait_ns);
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
         // The leader's barriers count both CTAs' loads; the other CTA meets it
@@ -561,11 +575,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
         bool ok = true;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
           for (int kb = 0; kb < kblocks; ++kb) {
-            ok = f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull) &&
-                 f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty);
+            ok = f8_wait(&full[stage], phase, abort_flag, err, kErrTimeoutFull, s.wait_ns) &&
+                 f8_wait(&acc_empty[buf], buf_phase ^ 1, abort_flag, err, kErrTimeoutAccEmpty, s.wait_ns);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
               f8_settle(acc_full, 2, buf, buf_phase);
+              f8_settle(empty, STAGES, stage, phase);
               break;
             }
             tc_fence_after();
@@ -621,7 +636,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
         const float f = a1 * w1;
         a1 = a2, w1 = w2;
         if (kb + 2 < kblocks) a2 = __ldg(sa + kb + 2), w2 = __ldg(sw + kb + 2);
-        ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull));
+        ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull, s.wait_ns));
         if (!ok) break;
         tc_fence_after();
         const float2 ff = make_float2(f, f);

@@ -276,10 +276,10 @@ extern "C" VD_API int vdk_quantize_fp8_weight(const void* w, int64_t ld_w, int64
   });
 }
 
-extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale,
-                                     const void* w, int64_t ld_w, const float* w_scale, int64_t ld_w_scale, int64_t M,
-                                     int64_t N, int64_t K, const float* bias, void* out, int64_t ld_out, int out_dtype,
-                                     int* status, void* stream, char* err, size_t errlen) {
+static int fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale, const void* w, int64_t ld_w,
+                      const float* w_scale, int64_t ld_w_scale, int64_t M, int64_t N, int64_t K, const float* bias,
+                      void* out, int64_t ld_out, int out_dtype, int* status, uint64_t wait_ns, int stall_after,
+                      void* stream, char* err, size_t errlen) {
   return guarded_call(err, errlen, [&] {
     need(M >= 0 && N >= 1 && K >= 1, "need M >= 0, N >= 1 and K >= 1");
     need(M <= (int64_t(1) << 30) && N <= 65535ll * 32 && K <= (int64_t(1) << 30), "a dimension is too large");
@@ -299,6 +299,8 @@ extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a
     s.out = out;
     s.ld_out = ld_out;
     s.out_aligned = rows16(out, ld_out, out_dtype);
+    s.wait_ns = wait_ns;
+    s.stall_after = stall_after;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     by_type(out_dtype, [&](auto tag) {
       using O = decltype(tag);
@@ -322,6 +324,27 @@ extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a
       else launch_f8_pair<O>(a, ld_a, w, ld_w, s, out_dtype, status, st);
     });
   });
+}
+
+extern "C" VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale,
+                                     const void* w, int64_t ld_w, const float* w_scale, int64_t ld_w_scale, int64_t M,
+                                     int64_t N, int64_t K, const float* bias, void* out, int64_t ld_out, int out_dtype,
+                                     int* status, void* stream, char* err, size_t errlen) {
+  return fp8_linear(a, ld_a, a_scale, ld_a_scale, w, ld_w, w_scale, ld_w_scale, M, N, K, bias, out, ld_out, out_dtype,
+                    status, VD_WAIT_TIMEOUT_NS, -1, stream, err, errlen);
+}
+
+extern "C" VD_API int vdk_fp8_linear_stalled(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale,
+                                             const void* w, int64_t ld_w, const float* w_scale, int64_t ld_w_scale,
+                                             int64_t M, int64_t N, int64_t K, const float* bias, void* out,
+                                             int64_t ld_out, int out_dtype, int* status, int64_t wait_limit_us,
+                                             int stall_after, void* stream, char* err, size_t errlen) {
+  if (wait_limit_us < 1 || wait_limit_us > 2000000 || stall_after < -1) {
+    put_err(err, errlen, "need 1 <= wait_limit_us <= 2e6 and stall_after >= -1");
+    return VD_EINVAL;
+  }
+  return fp8_linear(a, ld_a, a_scale, ld_a_scale, w, ld_w, w_scale, ld_w_scale, M, N, K, bias, out, ld_out, out_dtype,
+                    status, static_cast<uint64_t>(wait_limit_us) * 1000, stall_after, stream, err, errlen);
 }
 
 extern "C" VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, const void* h, int64_t ld_h, int h_dtype,
