@@ -652,3 +652,20 @@ def test_offsets_past_32_bits():
     v.copy_(heads)
     got, _ = ops.rotary(v, None, pos, plan, q_out=v)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_logprobs_bounds_that_rise_many_times(dt):
+    """Rows of more than a hundred batches whose maxima keep rising: every doubling of what has been read raises the
+    bound on the alternatives; the answer is the sorted one each time."""
+    vocab = 1_050_000
+    g = gen(31)
+    ramp = torch.linspace(0, 6, vocab, device="cuda")
+    x = (randn(g, 4, vocab) + ramp).to(DT[dt])
+    x = x.repeat(150, 1) if dt == "bf16" else x.repeat(75, 1)
+    ids = torch.zeros(x.shape[0], 1, dtype=torch.int64, device="cuda")
+    first = check_logprobs(x[:4], ids[:4], 64, 1.0)
+    for _ in range(5):
+        r = ops.token_logprobs(x, ids, top=64)
+        for i in range(0, x.shape[0], 4):
+            assert torch.equal(r.top_ids[i:i + 4], first.top_ids)

@@ -207,7 +207,7 @@ struct LpShared {
   uint64_t kept[kLpCap];
   uint64_t best[kLpMaxTop];  // this CTA's alternatives, largest first
   uint64_t group[kLpGroups];
-  uint64_t bound;
+  uint64_t bound[2];
   int count, kept_count;
   int hist[256];
   int above;
@@ -222,8 +222,10 @@ struct LpShared {
 };
 
 // The k-th largest of the 64 groups' largest keys (a group is kLpGroupSize threads):
-// at least k entries reach it.  0 where fewer groups have an entry.
-__device__ __forceinline__ uint64_t lp_group_bound(LpShared& sh, uint64_t best, int k) {
+// at least k entries reach it.  0 where fewer groups have an entry.  `word`: a
+// thread may still read the call before's result when another begins this call,
+// so calls with no barrier of the caller's between them take the two words in turn.
+__device__ __forceinline__ uint64_t lp_group_bound(LpShared& sh, uint64_t best, int k, int word) {
 #pragma unroll
   for (int o = kLpGroupSize / 2; o > 0; o >>= 1) {
     const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
@@ -231,7 +233,7 @@ __device__ __forceinline__ uint64_t lp_group_bound(LpShared& sh, uint64_t best, 
   }
   const int group = threadIdx.x / kLpGroupSize, in_group = threadIdx.x % kLpGroupSize;
   if (in_group == 0) sh.group[group] = best;
-  if (threadIdx.x == 0) sh.bound = 0;
+  if (threadIdx.x == 0) sh.bound[word] = 0;
   __syncthreads();
   // A group's threads count the keys above its own.
   const uint64_t mine = sh.group[group];
@@ -240,9 +242,9 @@ __device__ __forceinline__ uint64_t lp_group_bound(LpShared& sh, uint64_t best, 
   for (int i = 0; i < kLpGroups; i += kLpGroupSize) larger += sh.group[i + in_group] > mine;
 #pragma unroll
   for (int o = kLpGroupSize / 2; o > 0; o >>= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
-  if (larger == k - 1 && mine != 0) sh.bound = mine;  // keys are distinct
+  if (larger == k - 1 && mine != 0) sh.bound[word] = mine;  // keys are distinct
   __syncthreads();
-  return sh.bound;
+  return sh.bound[word];
 }
 
 // The k largest of get(0) .. get(n - 1), n <= kLpCap, into sh.best (0 past the last).
@@ -251,7 +253,7 @@ __device__ __forceinline__ void lp_select(LpShared& sh, int n, int k, Get&& get)
   uint64_t best = 0;
   for (int i = threadIdx.x; i < n; i += kLpThreads) best = get(i) > best ? get(i) : best;
   if (threadIdx.x == 0) sh.kept_count = 0;
-  const uint64_t bound = lp_group_bound(sh, best, k);
+  const uint64_t bound = lp_group_bound(sh, best, k, 0);
   for (int i = threadIdx.x; i < n; i += kLpThreads) {
     const uint64_t key = get(i);
     if (key != 0 && key >= bound) sh.kept[atomicAdd(&sh.kept_count, 1)] = key;
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
         // The thread's largest entry, the first of equal ones.
         uint64_t best = 0;
         if (bm > -INFINITY) best = lp_key(bm, static_cast<uint32_t>(id_of(base + tid, __ffs(b.reaching(top, bm)) - 1)));
-        bound = lp_group_bound(sh, best, k);
+        bound = lp_group_bound(sh, best, k, 0);
         if (bound) bound_x = lp_key_value(bound);
       }
       if (bm >= bound_x) collect(b, top, base + tid);
@@ -361,7 +363,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       // where less than half as much is left.
       if (++batches > 1 && (batches & (batches - 1)) == 0 &&
           ((end - base) / (kLpThreads * kLpUnroll) - 1) * 2 >= batches) {
-        const uint64_t higher = lp_group_bound(sh, st.m > -INFINITY ? lp_key(st.m, 0xffffffffu - tid) : 0, k);
+        const uint64_t higher = lp_group_bound(sh, st.m > -INFINITY ? lp_key(st.m, 0xffffffffu - tid) : 0, k,
+                                               (31 - __clz(batches)) & 1);
         if (higher != 0 && (higher | 0xffffffffu) > (bound | 0xffffffffu)) {
           bound = higher & ~0xffffffffull;
           bound_x = lp_key_value(bound);
@@ -409,11 +412,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
           while (bin > 0 && sum + sh.hist[bin] < k) sum += sh.hist[bin--];
           sh.above = sum;
           sh.count = sum + sh.hist[bin];
-          sh.bound = prefix | (static_cast<uint64_t>(bin) << shift);
+          sh.bound[0] = prefix | (static_cast<uint64_t>(bin) << shift);
         }
         __syncthreads();
         above = sh.above;
-        prefix = sh.bound;
+        prefix = sh.bound[0];
         const int reach = sh.count;
         __syncthreads();
         if (reach <= kLpCap) break;
