@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       send = sh.best;
       found = k;
     }
+    __syncwarp();  // the aligned barrier wants whole warps, and the loops and branches above split them
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA runs
     if (k > 0)
       for (int i = tid; i < found; i += kLpThreads)
