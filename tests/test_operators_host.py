@@ -192,3 +192,32 @@ def test_limits_of_the_failure_path_entry():
     for limit, stall in ((0, 0), (-1, 0), (2000001, 0), (1000, -2)):
         rc, msg = call("vdk_fp8_linear_stalled", *args, limit, stall)
         assert rc == _abi.VD_EINVAL and msg
+
+
+def test_c_entries_refuse_pointers_off_their_element():
+    """A kernel would fault on them; every pointer that one dereferences is looked at before a launch."""
+    F, H = FAKE, _abi.VdkRotaryHeads
+    # Far apart, so that nothing overlaps.
+    A, B, C, D, G, O = (F + (i << 20) for i in range(6))
+    quant = ["vdk_quantize_fp8", A, 128, B, 128, 4, 2, 128, 0, C, 128, D, 1]
+    weight = ["vdk_quantize_fp8_weight", A, 128, 2, 128, 2, C, 128, D, 1]
+    linear = ["vdk_fp8_linear", A, 128, B, 1, C, 128, D, 1, 4, 4, 128, G, O, 4, 0, F - 64]
+    norm = ["vdk_block_norm", A, 8, 0, B, 8, 2, C, D, 2, 8, 1, 1.0, 1.0, G, 1e-6, 0, 2, 8, O, 8, O + (1 << 20), 8, 0, None,
+            0]
+    norm8 = norm[:23] + [3, F - 64, 1]
+    logp = ["vdk_token_logprobs", A, 20, 2, 20, 0, 1.0, B, 1, 3, C, D, G, O, O + (1 << 20)]
+    cases = [(quant, 1, 1), (quant, 3, 1), (quant, 11, 2), (weight, 1, 2), (weight, 8, 1), (linear, 3, 2), (linear, 7, 2),
+             (linear, 12, 2), (linear, 13, 1), (linear, 16, 2), (norm, 1, 1), (norm, 4, 2), (norm, 7, 2), (norm, 8, 2),
+             (norm, 14, 2), (norm, 19, 2), (norm, 21, 1), (norm8, 24, 2), (logp, 1, 1), (logp, 7, 4), (logp, 10, 2),
+             (logp, 11, 2), (logp, 12, 2), (logp, 13, 2), (logp, 14, 2)]
+    for args, at, off in cases:
+        bad = list(args)
+        assert isinstance(bad[at], int) and bad[at] >= F - 64, (args, at)
+        bad[at] += off
+        rc, msg = call(*bad)
+        assert rc == _abi.VD_EINVAL and "aligned" in msg, (args[0], at, rc, msg)
+    for heads, pos, bits, turns in ((H(A + 1, B, 128, 64, 128, 64, 2), None, 0, C), (H(A, B + 1, 128, 64, 128, 64, 2), None, 0, C),
+                                    (H(A, B, 128, 64, 128, 64, 2), D + 2, 32, C), (H(A, B, 128, 64, 128, 64, 2), D + 4, 64, C),
+                                    (H(A, B, 128, 64, 128, 64, 2), None, 0, C + 4)):
+        rc, msg = call("vdk_rotary", heads, None, 3, 64, 64, 0, 0, 0, pos, bits, 0, turns, 1.0)
+        assert rc == _abi.VD_EINVAL and "aligned" in msg, msg

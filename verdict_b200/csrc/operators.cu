@@ -31,6 +31,16 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 int elem_bytes(int dtype) { return dtype == VDK_FP32 ? 4 : 2; }
 
+// What a kernel dereferences has to lie on its element's boundary.
+template <class T>
+void need_aligned(const T* p, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % alignof(T)) fail(VD_EINVAL, std::string(what) + " is not aligned to its type");
+}
+void need_aligned(const void* p, int dtype, const char* what) {
+  const int bytes = dtype == VDK_FP8 ? 1 : elem_bytes(dtype);
+  if (reinterpret_cast<uintptr_t>(p) % bytes) fail(VD_EINVAL, std::string(what) + " is not aligned to its type");
+}
+
 // Rows of `dtype` that all start on a 16-byte boundary.
 bool rows16(const void* p, int64_t ld, int dtype) { return aligned16(p) && ld * elem_bytes(dtype) % 16 == 0; }
 
@@ -227,6 +237,9 @@ extern "C" VD_API int vdk_quantize_fp8(const void* x, int64_t ld_x, const void* 
          "a row stride is smaller than its row");
     if (rows == 0) return;
     need(x && q && scale, "null buffer");
+    need_aligned(x, dtype, "x");
+    need_aligned(gate, dtype, "gate");
+    need_aligned(scale, "scale");
     QuantizeParams p{};
     p.x = x, p.gate = gate;
     p.ld_x = ld_x, p.ld_gate = ld_gate, p.ld_q = ld_q, p.ld_scale = ld_scale;
@@ -265,6 +278,8 @@ extern "C" VD_API int vdk_quantize_fp8_weight(const void* w, int64_t ld_w, int64
          "need 1 <= rows <= 8388480 and 1 <= cols < 2^31 - 128");
     need(ld_w >= cols && ld_q >= cols && ld_scale >= (cols + 127) / 128, "a row stride is smaller than its row");
     need(w && q && scale, "null buffer");
+    need_aligned(w, dtype, "w");
+    need_aligned(scale, "scale");
     const dim3 grid(static_cast<unsigned>((cols + 127) / 128), static_cast<unsigned>((rows + 127) / 128));
     by_type(dtype, [&](auto tag) {
       using T = decltype(tag);
@@ -291,6 +306,11 @@ static int fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t
     need(a && w && a_scale && w_scale && out, "null buffer");
     need(aligned16(a) && ld_a % 16 == 0 && aligned16(w) && ld_w % 16 == 0,
          "rows of a and w must start on 16-byte boundaries");
+    need_aligned(a_scale, "a_scale");
+    need_aligned(w_scale, "w_scale");
+    need_aligned(bias, "bias");
+    need_aligned(out, out_dtype, "out");
+    need_aligned(status, "status");
     F8Shape s{};
     s.M = static_cast<int>(M), s.N = static_cast<int>(N), s.K = static_cast<int>(K);
     s.sa = a_scale, s.sw = w_scale;
@@ -373,6 +393,14 @@ extern "C" VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, c
     need(y || h, "need a block output or a residual");
     need(h_out || z, "nothing to write");
     need(!z || z_dtype != VDK_FP8 || (z_scale && ld_z_scale >= kb), "8-bit z needs z_scale with a row per token");
+    need_aligned(y, y_dtype, "y");
+    need_aligned(h, h_dtype, "h");
+    need_aligned(gate, gate_dtype, "gate");
+    need_aligned(post_gain, "post_gain");
+    need_aligned(pre_gain, "pre_gain");
+    need_aligned(h_out, h_dtype, "h_out");
+    need_aligned(z, z_dtype, "z");
+    need_aligned(z_scale, "z_scale");
     BlockNormParams p{};
     p.y = y, p.h = h, p.post = post_gain, p.gate = gate;
     p.gate_f32 = gate_dtype == VDK_FP32;
@@ -504,6 +532,8 @@ extern "C" VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_hea
       if (!v) return;
       need(v->heads >= 1 && v->heads <= 65536, "heads must be from 1 to 65536");
       need(tokens == 0 || (v->in && v->out), "null buffer");
+      need_aligned(v->in, dtype, "heads");
+      need_aligned(v->out, dtype, "output heads");
       need(v->in_token >= 0 && v->in_head >= 0 && v->out_token >= 0 && v->out_head >= 0, "negative stride");
       // Output rows of head_dim lie apart: heads within a token, or tokens within a head.
       const int64_t hs = v->out_head, ts = v->out_token;
@@ -520,6 +550,9 @@ extern "C" VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_hea
     need(heads * head_dim <= (int64_t(1) << 28), "too many heads");
     if (tokens == 0) return;
     need(turns != nullptr, "null buffer");
+    need_aligned(turns, "turns");
+    need(reinterpret_cast<uintptr_t>(positions) % (positions_bits == 64 ? 8 : 4) == 0,
+         "positions are not aligned to their type");
     p.positions = positions;
     p.positions64 = positions_bits == 64;
     p.first_position = first_position;
@@ -561,7 +594,13 @@ extern "C" VD_API int vdk_token_logprobs(const void* logits, int64_t ld, int64_t
     need(logits != nullptr, "null buffer");
     need(n_targets == 0 || (targets && logprobs), "targets need their ids and an output");
     need(top == 0 || (top_ids && top_logprobs), "alternatives need their outputs");
-    need(reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype) == 0, "logits are not aligned to their type");
+    need_aligned(logits, dtype, "logits");
+    need_aligned(targets, "targets");
+    need_aligned(logprobs, "logprobs");
+    need_aligned(entropy, "entropy");
+    need_aligned(lse, "lse");
+    need_aligned(top_ids, "top_ids");
+    need_aligned(top_logprobs, "top_logprobs");
     static_assert(VDK_LOGPROBS_MAX_TOP == kLpMaxTop, "");
     LogprobParams p{};
     p.logits = logits;
