@@ -221,3 +221,9 @@ def test_c_entries_refuse_pointers_off_their_element():
                                     (H(A, B, 128, 64, 128, 64, 2), None, 0, C + 4)):
         rc, msg = call("vdk_rotary", heads, None, 3, 64, 64, 0, 0, 0, pos, bits, 0, turns, 1.0)
         assert rc == _abi.VD_EINVAL and "aligned" in msg, msg
+
+
+def test_quantize_row_count_does_not_wrap():
+    # rows * blocks is 4 modulo 2^64
+    rc, msg = call("vdk_quantize_fp8", FAKE, 512, None, 0, 0, (1 << 62) + 1, 512, 0, 2 * FAKE, 512, 3 * FAKE, 4)
+    assert rc == _abi.VD_EINVAL and "2^31" in msg

@@ -232,7 +232,7 @@ extern "C" VD_API int vdk_quantize_fp8(const void* x, int64_t ld_x, const void* 
     need(act >= VDK_ACT_NONE && act <= VDK_ACT_SILU, "unknown activation");
     need(gate || act == VDK_ACT_NONE, "an activation needs a gate");
     const int64_t col_blocks = (cols + 127) / 128;
-    need(rows * col_blocks <= kMaxInt, "rows * ceil(cols / 128) must be below 2^31");
+    need(rows <= kMaxInt / col_blocks, "rows * ceil(cols / 128) must be below 2^31");
     need(ld_x >= cols && ld_q >= cols && ld_scale >= col_blocks && (!gate || ld_gate >= cols),
          "a row stride is smaller than its row");
     if (rows == 0) return;
