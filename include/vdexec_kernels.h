@@ -186,8 +186,9 @@ VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, const void* 
 
 /*
  * Rotary frequencies for vdk_rotary: turns per position of each pair in 64-bit
- * fixed point (frequency / 2 pi * 2^64, whole turns dropped) and the factor on
- * the rotated values.  Host only.  Pair i turns theta^(-2 i / rotary_dim)
+ * fixed point (frequency / 2 pi * 2^64, whole turns dropped, within 4 units for
+ * frequencies of up to one radian) and the factor on the rotated values.  Host
+ * only.  Pair i turns theta^(-2 i / rotary_dim)
  * radians per position, then by `scaling`:
  *   VDK_ROPE_LINEAR   args {factor}: divided by factor
  *   VDK_ROPE_NTK      args {factor}: theta * factor^(d / (d - 2)) as the base
@@ -223,7 +224,9 @@ typedef struct vdk_rotary_heads {
  * (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved, of the first
  * rotary_dim columns of each head turn by positions[token] * turns[i]
  * (inverse: back); the other columns are copied.  positions: device int32 or
- * int64, any value, or NULL: first_position + token.  turns: device.
+ * int64, any value, or NULL: first_position + token; what turns[i] is off by is
+ * multiplied by the position (2^-62 of a turn each: below fp32's rounding of
+ * the cosines up to position 2^37).  turns: device.
  */
 VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_heads* k, int64_t tokens, int head_dim,
                       int rotary_dim, int dtype, int interleaved, int inverse, const void* positions,

@@ -669,3 +669,26 @@ def test_logprobs_bounds_that_rise_many_times(dt):
         r = ops.token_logprobs(x, ids, top=64)
         for i in range(0, x.shape[0], 4):
             assert torch.equal(r.top_ids[i:i + 4], first.top_ids)
+
+
+@pytest.mark.parametrize("scaling", [
+    None, {"type": "linear", "factor": 4.0}, {"type": "ntk", "factor": 8.0},
+    {"type": "yarn", "factor": 4.0, "original_max_position": 4096},
+    {"type": "llama3", "factor": 8.0, "original_max_position": 8192, "low_freq_factor": 1.0, "high_freq_factor": 4.0}])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_far_positions_against_the_formula(scaling, inverse):
+    """Frequencies from their formulas, not from the plan: a turn is off by at most 2^-62 per position."""
+    from rotary_reference import fraction_of_a_turn, turns_per_position
+    plan = ops.RotaryPlan(64, theta=1e6, scaling=scaling)
+    pos = [1, 131071, (1 << 31) - 1, 1 << 33, (1 << 37) - 5, -(1 << 37), (1 << 45) + 12345]
+    q = randn(gen(14), len(pos), 2, 64)
+    out, _ = ops.rotary(q, None, torch.tensor(pos, device="cuda"), plan, inverse=inverse)
+    turns = turns_per_position(64, 1e6, scaling)
+    frac = [[fraction_of_a_turn(p, t) for t in turns] for p in pos]
+    ang = 2 * math.pi * torch.tensor(frac, dtype=torch.float64, device="cuda")[:, None]
+    c, s = ang.cos() * plan.factor, ang.sin() * plan.factor * (-1 if inverse else 1)
+    a, b = q.double()[..., :32], q.double()[..., 32:]
+    ref = torch.cat([a * c - b * s, b * c + a * s], -1)
+    mag = torch.cat([a.abs() + b.abs()] * 2, -1)
+    off = 2 * math.pi * torch.tensor(pos, dtype=torch.float64, device="cuda").abs()[:, None, None] * 2.0 ** -62
+    within(out, ref, rotary_bound(ref, mag, plan, torch.float32) + off * plan.factor * mag)

@@ -2,11 +2,13 @@
 
 import ctypes
 import math
+from decimal import Decimal
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
+from rotary_reference import fraction_of_a_turn, turns_per_position  # noqa: E402
 from verdict_b200 import _abi, ops  # noqa: E402
 
 
@@ -227,3 +229,21 @@ def test_quantize_row_count_does_not_wrap():
     # rows * blocks is 4 modulo 2^64
     rc, msg = call("vdk_quantize_fp8", FAKE, 512, None, 0, 0, (1 << 62) + 1, 512, 0, 2 * FAKE, 512, 3 * FAKE, 4)
     assert rc == _abi.VD_EINVAL and "2^31" in msg
+
+
+SCALINGS = [
+    None, {"type": "linear", "factor": 3.0}, {"type": "ntk", "factor": 8.0},
+    {"type": "yarn", "factor": 4.0, "original_max_position": 4096},
+    {"type": "llama3", "factor": 8.0, "original_max_position": 8192, "low_freq_factor": 1.0, "high_freq_factor": 4.0},
+    {"type": "divisors", "divisors": [1.0 + i / 7 for i in range(48)]}]
+
+
+@pytest.mark.parametrize("scaling", SCALINGS)
+@pytest.mark.parametrize("rd,theta", [(96, 1e4), (96, 1e6), (96, 5e5)])
+def test_rotary_turns_have_all_their_64_bits(rd, theta, scaling):
+    """Against 70 digits.  In units of 2^-64 of a turn, at up to 0.16 turns: half a unit for the rounding, and a long
+    double's 2^-64 relative (0.16 units) for each of at most ten operations on the way (the power counts for two)."""
+    turns, _ = ops.rotary_turns(rd, theta, scaling)
+    for got, want in zip(turns, turns_per_position(rd, theta, scaling)):
+        off = fraction_of_a_turn(1, Decimal(got) / 2 ** 64 - want) * 2.0 ** 64
+        assert abs(off) <= 4, off

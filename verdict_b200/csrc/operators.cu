@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <limits>
 #include <string>
 #include <type_traits>
 
@@ -462,23 +463,27 @@ extern "C" VD_API int vdk_rotary_turns(double theta, int rotary_dim, int scaling
     need(turns && factor, "null buffer");
     need(scaling == VDK_ROPE_NONE || args, "the scaling needs its arguments");
     need(scaling != VDK_ROPE_DIVISORS || divisors, "the scaling needs one divisor per pair");
-    const double pi = 3.141592653589793238462643383279502884;
+    // A turn in 64 bits wants more than a double's 53 at every step up to it:
+    // the position multiplies what is lost here.
+    using real = long double;
+    const real two_pi = 6.283185307179586476925286766559005768L;
     const int half = rotary_dim / 2;
     const double d = rotary_dim;
-    double m = 1.0, base = theta;
+    double m = 1.0;
+    real base = theta;
     const double f = scaling != VDK_ROPE_NONE ? args[0] : 1.0;
     if (scaling != VDK_ROPE_NONE && scaling != VDK_ROPE_DIVISORS)
       need(std::isfinite(f) && f >= 1.0, "the scaling factor must be at least 1");
     double lo = 0.0, hi = 0.0;
     if (scaling == VDK_ROPE_NTK) {
       need(rotary_dim > 2, "this scaling needs rotary_dim > 2");
-      base = theta * std::pow(f, d / (d - 2.0));
+      base = theta * std::pow(static_cast<real>(f), static_cast<real>(d) / (d - 2.0));
     } else if (scaling == VDK_ROPE_YARN) {
       const double orig = args[1], fast = args[2], slow = args[3];
       need(orig > 0.0 && fast > slow && slow > 0.0, "need original_max_position > 0 and beta_fast > beta_slow > 0");
       need(theta != 1.0, "this scaling needs theta != 1");
       auto dim = [&](double turns_over) {
-        return d * std::log(orig / (turns_over * 2.0 * pi)) / (2.0 * std::log(theta));
+        return d * std::log(orig / (turns_over * static_cast<double>(two_pi))) / (2.0 * std::log(theta));
       };
       lo = std::max(std::floor(dim(fast)), 0.0);
       hi = std::min(std::ceil(dim(slow)), d - 1.0);
@@ -489,24 +494,24 @@ extern "C" VD_API int vdk_rotary_turns(double theta, int rotary_dim, int scaling
       m = args[0];
       need(std::isfinite(m) && m > 0.0, "the factor on the rotated values must be positive");
     }
+    const real zero = 0, one = 1;
     for (int i = 0; i < half; ++i) {
-      double r = std::pow(base, -2.0 * i / d);  // radians per position
+      real r = std::pow(base, static_cast<real>(-2 * i) / rotary_dim);  // radians per position
       if (scaling == VDK_ROPE_LINEAR) {
         r /= f;
       } else if (scaling == VDK_ROPE_YARN) {
-        const double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
-        r = r / f * ramp + r * (1.0 - ramp);
+        const real ramp = std::min(std::max((i - static_cast<real>(lo)) / std::max(hi - lo, 0.001), zero), one);
+        r = r / f * ramp + r * (one - ramp);
       } else if (scaling == VDK_ROPE_LLAMA3) {
-        const double t = std::min(std::max((args[1] * r / (2.0 * pi) - args[2]) / (args[3] - args[2]), 0.0), 1.0);
-        r = (1.0 - t) * r / f + t * r;
+        const real t = std::min(std::max((args[1] * r / two_pi - args[2]) / (args[3] - args[2]), zero), one);
+        r = (one - t) * r / f + t * r;
       } else if (scaling == VDK_ROPE_DIVISORS) {
         need(std::isfinite(divisors[i]) && divisors[i] > 0.0, "divisors must be positive");
         r /= divisors[i];
       }
-      const double t = r / (2.0 * pi);
-      const double frac = t - std::floor(t);
-      // frac < 1, and a double has 53 bits: the product is exact, below 2^64.
-      turns[i] = static_cast<uint64_t>(std::ldexp(frac, 64));
+      const real t = r / two_pi;
+      const real scaled = std::round(std::ldexp(t - std::floor(t), 64));
+      turns[i] = scaled < std::ldexp(one, 64) ? static_cast<uint64_t>(scaled) : 0;  // rounded up to a whole turn
     }
     *factor = static_cast<float>(m);
   });
