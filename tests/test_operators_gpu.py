@@ -692,3 +692,20 @@ def test_rotary_far_positions_against_the_formula(scaling, inverse):
     mag = torch.cat([a.abs() + b.abs()] * 2, -1)
     off = 2 * math.pi * torch.tensor(pos, dtype=torch.float64, device="cuda").abs()[:, None, None] * 2.0 ** -62
     within(out, ref, rotary_bound(ref, mag, plan, torch.float32) + off * plan.factor * mag)
+
+
+def test_rotary_cosines_and_sines_near_quarter_turns():
+    """Rotating (1, 0) gives the cosine and the sine themselves.  The turn is reduced before it is rounded, so each is
+    right to a few units in its own last place, small ones beside a half or quarter turn too: 2^-24 for the rounded rest,
+    one unit (at most 2^-23) for the function."""
+    plan = ops.RotaryPlan(64, theta=1e4)
+    pos = torch.randint(0, 131072, (4096,), generator=gen(41), device="cuda")
+    q = torch.zeros(4096, 1, 64, device="cuda")
+    q[..., :32] = 1
+    out, _ = ops.rotary(q, None, pos, plan)
+    mine = [t % (1 << 64) for t in plan.turns.tolist()]
+    ang = 2 * math.pi * torch.tensor([[((p * t) % (1 << 64)) / 2.0 ** 64 for t in mine] for p in pos.tolist()],
+                                     dtype=torch.float64, device="cuda")
+    want = torch.cat([ang.cos(), ang.sin()], -1)[:, None]
+    within(out, want, 4 * U * want.abs() + 1e-12)
+    assert (want.abs() < 1e-4).sum() > 10  # some do lie there
