@@ -120,6 +120,8 @@ VD_API int vdk_attention_noalloc(const void* qkv, int64_t ld_qkv, int64_t q_col0
  * stream capture.  Buffers belong to the current device and must stay valid
  * until the work has run.  Arguments are checked before anything is launched
  * (VD_EINVAL); zero rows are no work and no error.  Strides count elements.
+ * Outputs share no memory with each other or with inputs, save where an entry
+ * says that one may be the same rows as an input.
  */
 
 /*
@@ -171,10 +173,11 @@ VD_API int vdk_fp8_linear_stalled(const void* a, int64_t ld_a, const float* a_sc
  * rmsnorm(x) = x / sqrt(mean(x^2) + eps); plus_one: gains are 1 + gain.
  * y (VDK_FP16 / BF16 / FP32, or NULL: u = 0), h (fp32 or y's type, or NULL:
  * 0), gate (fp32 or y's type, or NULL: 1) with strides that may be 0 to
- * broadcast (columns: 0 or 1); h_out has h's type (NULL: not stored) and may
- * be h itself.  z is VDK_FP16, BF16, FP32 or FP8; FP8 comes with z_scale
- * [rows, ceil(cols / 128)] as vdk_quantize_fp8 gives it; z and pre_gain NULL:
- * no second norm.  z is formed in fp32 from h_out before that is rounded.
+ * broadcast (columns: 0 or 1); h_out has h's type (NULL: not stored); h_out or
+ * z may be the rows of h, y or a gate with a value per element.  z is VDK_FP16,
+ * BF16, FP32 or FP8; FP8 comes with z_scale [rows, ceil(cols / 128)] as
+ * vdk_quantize_fp8 gives it; z and pre_gain NULL: no second norm.  z is formed
+ * in fp32 from h_out before that is rounded.
  */
 #define VDK_NORM_MAX_COLS 16384
 VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, const void* h, int64_t ld_h, int h_dtype,
@@ -211,7 +214,7 @@ VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, const void* 
 VD_API int vdk_rotary_turns(double theta, int rotary_dim, int scaling, const double* args, const double* divisors,
                             uint64_t* turns, float* factor, char* err, size_t errlen);
 
-/* Heads of vdk_rotary: [tokens, heads, head_dim] with unit stride in a head; out may be in. */
+/* Heads of vdk_rotary: [tokens, heads, head_dim] with unit stride in a head; out may be in's rows. */
 typedef struct vdk_rotary_heads {
   const void* in;
   void* out;

@@ -15,6 +15,7 @@
 #include "block_norm.cuh"
 #include "fp8_gemm.cuh"
 #include "host.hpp"
+#include "overlap.hpp"
 #include "quantize.cuh"
 #include "rotary.cuh"
 #include "token_logprobs.cuh"
@@ -40,6 +41,19 @@ void need_aligned(const T* p, const char* what) {
 void need_aligned(const void* p, int dtype, const char* what) {
   const int bytes = dtype == VDK_FP8 ? 1 : elem_bytes(dtype);
   if (reinterpret_cast<uintptr_t>(p) % bytes) fail(VD_EINVAL, std::string(what) + " is not aligned to its type");
+}
+
+// Matrix [rows, cols] of `dtype` with row stride ld.
+ByteRows matrix(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype) {
+  const int64_t bytes = dtype == VDK_FP8 ? 1 : elem_bytes(dtype);
+  return {p, cols * bytes, rows, ld * bytes};
+}
+
+// What one thread writes no other may read or write: an output lies apart from
+// everything else, or (where the kernel reads an element in the thread that
+// writes it) it is the same rows.
+void need_apart(const ByteRows& out, const ByteRows& other, const char* what, bool or_same = false) {
+  if (overlap(out, other) && !(or_same && same_rows(out, other))) fail(VD_EINVAL, std::string(what) + " overlap");
 }
 
 // Rows of `dtype` that all start on a 16-byte boundary.
@@ -241,6 +255,13 @@ extern "C" VD_API int vdk_quantize_fp8(const void* x, int64_t ld_x, const void* 
     need_aligned(x, dtype, "x");
     need_aligned(gate, dtype, "gate");
     need_aligned(scale, "scale");
+    const ByteRows mx = matrix(x, rows, cols, ld_x, dtype), mg = matrix(gate, rows, cols, ld_gate, dtype),
+                   mq = matrix(q, rows, cols, ld_q, VDK_FP8), ms = matrix(scale, rows, col_blocks, ld_scale, VDK_FP32);
+    need_apart(mq, mx, "q and x");
+    need_apart(mq, mg, "q and gate");
+    need_apart(ms, mx, "scale and x");
+    need_apart(ms, mg, "scale and gate");
+    need_apart(mq, ms, "q and scale");
     QuantizeParams p{};
     p.x = x, p.gate = gate;
     p.ld_x = ld_x, p.ld_gate = ld_gate, p.ld_q = ld_q, p.ld_scale = ld_scale;
@@ -281,6 +302,11 @@ extern "C" VD_API int vdk_quantize_fp8_weight(const void* w, int64_t ld_w, int64
     need(w && q && scale, "null buffer");
     need_aligned(w, dtype, "w");
     need_aligned(scale, "scale");
+    const ByteRows mw = matrix(w, rows, cols, ld_w, dtype), mq = matrix(q, rows, cols, ld_q, VDK_FP8),
+                   ms = matrix(scale, (rows + 127) / 128, (cols + 127) / 128, ld_scale, VDK_FP32);
+    need_apart(mq, mw, "q and w");
+    need_apart(ms, mw, "scale and w");
+    need_apart(mq, ms, "q and scale");
     const dim3 grid(static_cast<unsigned>((cols + 127) / 128), static_cast<unsigned>((rows + 127) / 128));
     by_type(dtype, [&](auto tag) {
       using T = decltype(tag);
@@ -312,6 +338,13 @@ static int fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t
     need_aligned(bias, "bias");
     need_aligned(out, out_dtype, "out");
     need_aligned(status, "status");
+    const ByteRows mo = matrix(out, M, N, ld_out, out_dtype);
+    need_apart(mo, matrix(a, M, K, ld_a, VDK_FP8), "out and a");
+    need_apart(mo, matrix(w, N, K, ld_w, VDK_FP8), "out and w");
+    need_apart(mo, matrix(a_scale, M, kb, ld_a_scale, VDK_FP32), "out and a_scale");
+    need_apart(mo, matrix(w_scale, (N + 127) / 128, kb, ld_w_scale, VDK_FP32), "out and w_scale");
+    need_apart(mo, ByteRows(bias, 4 * N), "out and bias");
+    need_apart(mo, ByteRows(status, 4), "out and status");
     F8Shape s{};
     s.M = static_cast<int>(M), s.N = static_cast<int>(N), s.K = static_cast<int>(K);
     s.sa = a_scale, s.sw = w_scale;
@@ -402,6 +435,23 @@ extern "C" VD_API int vdk_block_norm(const void* y, int64_t ld_y, int y_dtype, c
     need_aligned(h_out, h_dtype, "h_out");
     need_aligned(z, z_dtype, "z");
     need_aligned(z_scale, "z_scale");
+    // y, h and a gate with a value per element are read by the thread that
+    // writes the same element: an output may be one of them.
+    const ByteRows my = matrix(y, rows, cols, ld_y, y_dtype), mh = matrix(h, rows, cols, ld_h, h_dtype),
+                   mg = matrix(gate, rows, gate_col_stride ? cols : 1, gate_row_stride, gate_dtype),
+                   mo = matrix(h_out, rows, cols, ld_h_out, h_dtype), mz = matrix(z, rows, cols, ld_z, z_dtype),
+                   ms = matrix(z && z_dtype == VDK_FP8 ? z_scale : nullptr, rows, kb, ld_z_scale, VDK_FP32);
+    for (const ByteRows* o : {&mo, &mz, &ms}) {
+      if (!o->p) continue;
+      need_apart(*o, my, "an output and y", o != &ms);
+      need_apart(*o, mh, "an output and h", o != &ms);
+      need_apart(*o, mg, "an output and gate", o != &ms && gate_col_stride);
+      need_apart(*o, ByteRows(post_gain, 4 * cols), "an output and post_gain");
+      need_apart(*o, ByteRows(pre_gain, 4 * cols), "an output and pre_gain");
+    }
+    need_apart(mo, mz, "h_out and z");
+    need_apart(mo, ms, "h_out and z_scale");
+    need_apart(mz, ms, "z and z_scale");
     BlockNormParams p{};
     p.y = y, p.h = h, p.post = post_gain, p.gate = gate;
     p.gate_f32 = gate_dtype == VDK_FP32;
@@ -558,6 +608,23 @@ extern "C" VD_API int vdk_rotary(const vdk_rotary_heads* q, const vdk_rotary_hea
     need_aligned(turns, "turns");
     need(reinterpret_cast<uintptr_t>(positions) % (positions_bits == 64 ? 8 : 4) == 0,
          "positions are not aligned to their type");
+    const int64_t row = static_cast<int64_t>(head_dim) * es;
+    const auto rows_in = [&](const vdk_rotary_heads* v) {
+      return v ? ByteRows(v->in, row, tokens, v->in_token * es, v->heads, v->in_head * es) : ByteRows();
+    };
+    const auto rows_out = [&](const vdk_rotary_heads* v) {
+      return v ? ByteRows(v->out, row, tokens, v->out_token * es, v->heads, v->out_head * es) : ByteRows();
+    };
+    const ByteRows q_in = rows_in(q), k_in = rows_in(k), q_out = rows_out(q), k_out = rows_out(k);
+    need_apart(q_out, q_in, "queries and their output", true);
+    need_apart(k_out, k_in, "keys and their output", true);
+    need_apart(q_out, k_in, "keys and the queries' output");
+    need_apart(k_out, q_in, "queries and the keys' output");
+    need_apart(q_out, k_out, "the outputs");
+    for (const ByteRows* o : {&q_out, &k_out}) {
+      need_apart(*o, ByteRows(positions, tokens * (positions_bits / 8)), "an output and positions");
+      need_apart(*o, ByteRows(turns, rotary_dim / 2 * 8), "an output and turns");
+    }
     p.positions = positions;
     p.positions64 = positions_bits == 64;
     p.first_position = first_position;
@@ -606,6 +673,14 @@ extern "C" VD_API int vdk_token_logprobs(const void* logits, int64_t ld, int64_t
     need_aligned(lse, "lse");
     need_aligned(top_ids, "top_ids");
     need_aligned(top_logprobs, "top_logprobs");
+    const ByteRows outs[] = {ByteRows(n_targets ? logprobs : nullptr, rows * n_targets * 4), ByteRows(entropy, rows * 4),
+                             ByteRows(lse, rows * 4), ByteRows(top ? top_ids : nullptr, rows * top * 4),
+                             ByteRows(top ? top_logprobs : nullptr, rows * top * 4)};
+    for (int i = 0; i < 5; ++i) {
+      need_apart(outs[i], matrix(logits, rows, vocab, ld, dtype), "an output and logits");
+      need_apart(outs[i], ByteRows(n_targets ? targets : nullptr, rows * n_targets * 8), "an output and targets");
+      for (int j = 0; j < i; ++j) need_apart(outs[i], outs[j], "two outputs");
+    }
     static_assert(VDK_LOGPROBS_MAX_TOP == kLpMaxTop, "");
     LogprobParams p{};
     p.logits = logits;
