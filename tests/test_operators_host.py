@@ -247,3 +247,10 @@ def test_rotary_turns_have_all_their_64_bits(rd, theta, scaling):
     for got, want in zip(turns, turns_per_position(rd, theta, scaling)):
         off = fraction_of_a_turn(1, Decimal(got) / 2 ** 64 - want) * 2.0 ** 64
         assert abs(off) <= 4, off
+
+
+def test_logprobs_temperature_whose_exponent_factor_overflows_is_refused():
+    # 1 / temperature is an fp32 number, log2(e) / temperature is not
+    for t in (3.0e-39, 4.2e-39):
+        rc, msg = call("vdk_token_logprobs", FAKE, 20, 2, 20, 0, t, None, 0, 0, None, None, None, None, None)
+        assert rc == _abi.VD_EINVAL and "temperature" in msg, (t, rc, msg)
