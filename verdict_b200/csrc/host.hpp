@@ -55,18 +55,35 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-inline EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
+// cuTensorMapEncodeTiled, which wants a context current on the calling thread:
+// where no runtime call has made one so yet, that of the thread's device.
+struct EncodeTiled {
+  EncodeTiledFn fn = nullptr;
+  template <class... A>
+  CUresult operator()(const A&... a) const {
+    CUresult r = fn(a...);
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+      int dev = 0;
+      cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+      cuda_check(cudaSetDevice(dev), "cudaSetDevice");
+      r = fn(a...);
+    }
+    return r;
+  }
+};
+
+inline EncodeTiled encode_fn() {
+  static EncodeTiled encode;
   static std::once_flag once;
   std::call_once(once, [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
         q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
+      encode.fn = reinterpret_cast<EncodeTiledFn>(p);
   });
-  if (!fn) fail(VD_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  return fn;
+  if (!encode.fn) fail(VD_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  return encode;
 }
 
 }  // namespace vd
