@@ -77,3 +77,47 @@ def test_check_status_raises_once():
     assert e.value.code == _abi.VD_ECUDA
     ops.check_status()
     assert torch.equal(ops.fp8_linear(*a, *w), want)
+
+
+def test_every_thread_that_ran_products_learns_of_a_failure():
+    import threading
+    a, w = operands(5, 256, 1024)
+    want = ops.fp8_linear(*a, *w)
+    ran, go, told = threading.Barrier(3), threading.Barrier(3), []
+
+    def worker(slot):
+        ops.fp8_linear(*a, *w)
+        ran.wait(60)
+        go.wait(60)
+        try:
+            ops.check_status()
+        except _abi.VdError:
+            told.append(slot)
+        ops.check_status()  # once
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    ran.wait(60)
+    limited(a, w, torch.empty_like(want), ops._status_word(want.device), 1000, 0)
+    with pytest.raises(_abi.VdError):
+        ops.check_status()  # this thread asks first
+    go.wait(60)
+    for t in threads:
+        t.join(60)
+    assert sorted(told) == [0, 1]
+    # A thread that starts afterwards has nothing to learn.
+    late = []
+
+    def newcomer():
+        try:
+            ops.fp8_linear(*a, *w)
+            ops.check_status()
+        except _abi.VdError as e:
+            late.append(e)
+
+    t = threading.Thread(target=newcomer)
+    t.start()
+    t.join(60)
+    assert not late
+    ops.check_status()

@@ -50,8 +50,10 @@ MAX_TOP = 64
 
 _CODES = {torch.float16: _abi.VDK_FP16, torch.bfloat16: _abi.VDK_BF16, torch.float32: _abi.VDK_FP32}
 _NORM_CODES = {**_CODES, FP8: _abi.VDK_FP8, None: -1}
-_status: dict = {}
+_status: dict = {}     # device index -> the word that fp8_linear's kernels leave a code in
+_failures: dict = {}   # device index -> (how many codes check_status has found there, the last one)
 _status_lock = threading.Lock()
+_thread = threading.local()  # .seen: device index -> how many of those failures this thread knows of
 
 
 # ---------------------------------------------------------------------------
@@ -71,30 +73,47 @@ def quantize_fp8_weight(w: torch.Tensor):
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
-    word = _status.get(device.index)
-    if word is None:
-        with _status_lock:
-            word = _status.get(device.index)
-            if word is None:
-                word = torch.zeros(1, dtype=torch.int32, device=device)
-                torch.cuda.synchronize(device)  # zero before any stream's kernel sees it
-                _status[device.index] = word
+    index = device.index
+    try:
+        _thread.seen[index]
+        return _status[index]
+    except (AttributeError, KeyError):
+        pass
+    with _status_lock:
+        word = _status.get(index)
+        if word is None:
+            word = torch.zeros(1, dtype=torch.int32, device=device)
+            torch.cuda.synchronize(device)  # zero before any stream's kernel sees it
+            _status[index] = word
+        if not hasattr(_thread, "seen"):
+            _thread.seen = {}
+        _thread.seen.setdefault(index, _failures.get(index, (0, 0))[0])
     return word
 
 
 def check_status(device=None) -> None:
-    """Waits for the device and raises VdError if a pipeline wait of an earlier fp8_linear on it ran out."""
+    """Waits for the device and raises VdError if a pipeline wait of an earlier fp8_linear on it ran out.  Threads share
+    a device: one that has called fp8_linear there learns of every such failure since its first call, once, whichever
+    thread's call it was and whoever asked first."""
     index = torch.device(device).index if device is not None else None
     if index is None:
         index = torch.cuda.current_device()
     torch.cuda.synchronize(index)
-    word = _status.get(index)
-    if word is not None:
-        code = int(word.item())
-        if code:
+    with _status_lock:
+        count, code = _failures.get(index, (0, 0))
+        word = _status.get(index)
+        found = int(word.item()) if word is not None else 0
+        if found:
             word.zero_()
             torch.cuda.synchronize(index)
-            raise _abi.VdError(_abi.VD_ECUDA, f"a kernel reported device error {code}")
+            count, code = _failures[index] = (count + 1, found)
+        seen = getattr(_thread, "seen", {})
+        # A thread that only asks is told of what it finds itself.
+        new = count > seen.get(index, count - bool(found))
+        if index in seen:
+            seen[index] = count
+    if new:
+        raise _abi.VdError(_abi.VD_ECUDA, f"a kernel reported device error {code}")
 
 
 def fp8_linear(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
