@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -86,6 +87,8 @@ void check(const Tensor& t, const char* name, int64_t dims, unsigned types, cons
   if (t.dim() != dims) say(" must have " + std::to_string(dims) + " dimensions, got shape " + shape_of(t));
   if (t.requires_grad() && c10::GradMode::is_enabled())
     say(" requires a gradient: this operator has no backward pass");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
+    say(" carries a forward-mode tangent: this operator has no derivative");
   if (!t.is_contiguous()) {
     if (packed) say(" must be contiguous");
     if (t.size(-1) > 1 && t.stride(-1) != 1) say(" needs unit stride along its last dimension");
