@@ -32,3 +32,33 @@ def test_forward_mode_tangents_are_refused():
         with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # no_grad leaves forward mode on
             ops.quantize_fp8(d)
         ops.quantize_fp8(x)  # without a tangent
+
+
+def test_writes_count_in_the_tensors_version():
+    x = torch.randn(4, 256, device="cuda")
+    q, s = ops.quantize_fp8(x)
+    w, sw = ops.quantize_fp8_weight(x)
+    out = torch.empty(4, 4, device="cuda", dtype=torch.bfloat16)
+    h, heads, ko = x.clone(), x.clone().view(4, 4, 64), torch.empty(4, 4, 64, device="cuda")
+    before = [t._version for t in (out, h, heads, ko, x, q)]
+    ops.fp8_linear(q, s, w, sw, out=out)
+    ops.block_norm(x, h, in_place=True)
+    ops.rotary(heads, x.view(4, 4, 64), 0, ops.RotaryPlan(64), q_out=heads, k_out=ko)
+    after = [t._version for t in (out, h, heads, ko, x, q)]
+    assert [a - b for a, b in zip(after, before)] == [1, 1, 1, 1, 0, 0]
+    # So a tensor that autograd saved is missed when it is overwritten.
+    leaf = torch.ones(4, 256, device="cuda", requires_grad=True)
+    saved = torch.randn(4, 256, device="cuda")
+    product = (leaf * saved).sum()
+    ops.block_norm(x, saved, in_place=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    # Nothing is written: a residual that is handed through, no rows.
+    b = h._version
+    ops.block_norm(None, h, pre_gain=torch.ones(256, device="cuda"), in_place=True)
+    ops.block_norm(x[:0], h[:0], in_place=True)
+    assert h._version == b
+    with torch.inference_mode():
+        i = torch.zeros(4, 256, device="cuda")
+    ops.block_norm(x, i, in_place=True)
+    assert torch.equal(i, x)

@@ -116,6 +116,11 @@ int64_t ld16(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : up16(t.size
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
+// A tensor of the caller's was written: autograd and views saved for it see that.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor empty(at::IntArrayRef shape, ScalarType type, const Tensor& like) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
 }
@@ -241,6 +246,7 @@ PyObject* fp8_linear(PyObject* const* p) {  // a, a_scale, w, w_scale, bias, out
                             ld(out), out_code, static_cast<int*>(ptr(status)), s, e, len);
     });
   if (given) {
+    if (m) written(*given);
     Py_INCREF(p[6]);
     return p[6];
   }
@@ -311,6 +317,7 @@ PyObject* block_norm(PyObject* const* p) {
                             !pre ? 0 : out_code == VDK_FP8 ? ld16(z) : ld(z), pre ? out_code : 0,
                             scale.defined() ? static_cast<float*>(ptr(scale)) : nullptr, blocks(cols), s, e, n);
     });
+  if (rows && in_place && !keep) written(*h);
   PyObject* residual;
   if (keep || in_place) {
     residual = p[1];
@@ -384,6 +391,8 @@ PyObject* rotary(PyObject* const* p) {
                         static_cast<int>(rotary_dim), code(type_of(x)), interleaved, inverse, positions, bits, first,
                         static_cast<const uint64_t*>(ptr(turns)), factor, s, e, n);
     });
+  for (int i = 0; i < 2; ++i)
+    if (tokens && ins[i] && p[9 + i] != Py_None) written(outs[i]);
   return tuple(q ? &outs[0] : nullptr, k ? &outs[1] : nullptr);
 }
 
