@@ -709,3 +709,14 @@ def test_rotary_cosines_and_sines_near_quarter_turns():
     want = torch.cat([ang.cos(), ang.sin()], -1)[:, None]
     within(out, want, 4 * U * want.abs() + 1e-12)
     assert (want.abs() < 1e-4).sum() > 10  # some do lie there
+
+
+def test_negated_views_are_refused():
+    """Their memory holds the values with the other sign."""
+    x = torch.randn(4, 256, device="cuda")
+    neg = torch._neg_view(x)
+    assert torch.equal(neg, -x) and neg.data_ptr() == x.data_ptr()
+    for f in (lambda: ops.quantize_fp8(neg), lambda: ops.block_norm(neg, x), lambda: ops.token_logprobs(neg)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            f()
+    assert torch.equal(ops.block_norm(neg.resolve_neg(), x).residual, torch.zeros_like(x))

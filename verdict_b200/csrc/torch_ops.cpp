@@ -85,6 +85,7 @@ void check(const Tensor& t, const char* name, int64_t dims, unsigned types, cons
   if (like && t.device() != like->device()) say(" is on " + t.device().str() + ", expected " + like->device().str());
   if (!(type_of(t) & types)) say(std::string(" has unsupported dtype ") + c10::toString(t.scalar_type()));
   if (t.dim() != dims) say(" must have " + std::to_string(dims) + " dimensions, got shape " + shape_of(t));
+  if (t.is_neg()) say(" is a negated view: materialise it first (resolve_neg)");
   if (t.requires_grad() && c10::GradMode::is_enabled())
     say(" requires a gradient: this operator has no backward pass");
   if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
