@@ -10,6 +10,7 @@ no libcuda at link time.
 from __future__ import annotations
 
 import concurrent.futures
+import hashlib
 import importlib.util
 import os
 import shutil
@@ -28,6 +29,10 @@ OBJ = os.path.join(PKG, "_build")
 # The torch binding of verdict_b200/ops.py, built beside the library where torch is installed.
 TORCH_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
 TORCH_LIB = os.path.join(PKG, "_torch_ops.so")
+# What each was built from.
+HEADERS = [os.path.join(INCLUDE, "vdexec.h"), os.path.join(INCLUDE, "vdexec_kernels.h")]
+LIB_STAMP = os.path.join(OBJ, "libvdexec.stamp")
+TORCH_STAMP = os.path.join(OBJ, "torch_ops.stamp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -51,11 +56,43 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in DEPS if os.path.exists(p) and p != TORCH_SOURCE)
 
 
+def _digest(paths, *more: str) -> str:
+    h = hashlib.sha256()
+    for p in paths:
+        with open(p, "rb") as f:
+            h.update(hashlib.sha256(f.read()).digest())
+    for m in more:
+        h.update(m.encode() + b"\0")
+    return h.hexdigest()
+
+
+def _read(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read().strip()
+    except OSError:
+        return ""
+
+
+def _write(path: str, text: str) -> None:
+    with open(path, "w") as f:
+        f.write(text + "\n")
+
+
+def library_has_this_header() -> bool:
+    """Whether libvdexec.so was built with the C entries as include/ declares them now."""
+    return up_to_date() or _read(LIB_STAMP) == _digest(HEADERS)
+
+
+def _torch_digest() -> str:
+    """What the torch binding depends on: its source, the C entries it calls, and the torch and Python it is built for."""
+    import torch
+
+    return _digest([TORCH_SOURCE, *HEADERS], torch.__version__, str(torch.version.cuda), sys.implementation.cache_tag)
+
+
 def torch_up_to_date() -> bool:
-    if not os.path.exists(TORCH_LIB):
-        return False
-    t = os.path.getmtime(TORCH_LIB)
-    return all(os.path.getmtime(p) <= t for p in (TORCH_SOURCE, os.path.join(INCLUDE, "vdexec_kernels.h")))
+    return os.path.exists(TORCH_LIB) and _read(TORCH_STAMP) == _torch_digest()
 
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
@@ -76,8 +113,12 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
         cmd += ["-L", path]
     cmd += [TORCH_SOURCE, "-o", TORCH_LIB + ".tmp", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
             "-L", PKG, "-l:libvdexec.so", "-Wl,-rpath,$ORIGIN"]
+    digest = _torch_digest()
     _run(cmd, verbose)
+    os.makedirs(OBJ, exist_ok=True)
+    _write(TORCH_STAMP, "")  # until the new file is in place
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    _write(TORCH_STAMP, digest)
     return TORCH_LIB
 
 
@@ -95,12 +136,15 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
     os.makedirs(OBJ, exist_ok=True)
+    digest = _digest(HEADERS)
     objects = [os.path.join(OBJ, os.path.splitext(os.path.basename(src))[0] + ".o") for src in SOURCES]
     flags = [*NVCC_FLAGS, *(["-Xptxas=-v"] if verbose else []), "-I", INCLUDE, "-I", CSRC]
     with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
         list(pool.map(lambda so: _run([nvcc(), *flags, "-c", so[0], "-o", so[1]], verbose), zip(SOURCES, objects)))
     _run([nvcc(), *NVCC_FLAGS, "-shared", *objects, "-o", LIB + ".tmp"], verbose)
+    _write(LIB_STAMP, "")
     os.replace(LIB + ".tmp", LIB)
+    _write(LIB_STAMP, digest)
     return LIB
 
 

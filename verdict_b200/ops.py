@@ -18,7 +18,6 @@ from __future__ import annotations
 
 import ctypes
 import importlib
-import os
 import threading
 from typing import NamedTuple, Optional
 
@@ -29,14 +28,14 @@ from . import build as _build
 
 
 def _load():
-    """The torch binding (built first where it or the library is missing or stale); it loads libvdexec.so."""
+    """The torch binding (built first where it or the library is missing or stale); it loads libvdexec.so.  A binding
+    made for other C entries or another torch is never used: it would pass arguments that are read as others."""
     _abi.load()
+    if not _build.library_has_this_header():
+        raise RuntimeError("libvdexec.so was built from other headers and could not be rebuilt; run "
+                           "`python -m verdict_b200.build`")
     if not _build.torch_up_to_date():
-        try:
-            _build.build_torch_ops()
-        except Exception:
-            if not os.path.exists(_build.TORCH_LIB):
-                raise
+        _build.build_torch_ops()
     return importlib.import_module("verdict_b200._torch_ops")
 
 
