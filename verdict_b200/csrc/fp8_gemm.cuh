@@ -38,14 +38,13 @@ struct F8Shape {
 
 // mbar_wait with the clock read only after a run of polls: reading the global
 // timer takes longer than the k-block that most waits here are for.
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code,
                                         uint64_t limit_ns) {
   uint64_t t0 = 0;
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 32; ++i) {
-      if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+      if (mbar_try_wait(bar, parity)) return true;
       if (*abort_flag) return false;
     }
     const uint64_t t = globaltimer();
