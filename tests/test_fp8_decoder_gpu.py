@@ -174,3 +174,15 @@ def test_refusals_and_empty_input():
         Fp8Decoder(specs.preset("laya-bert"), {})
     with pytest.raises(ValueError):
         Fp8Decoder(specs.preset("onejev16-9b"), {})
+
+
+def test_the_model_stays_on_the_device_it_was_built_on():
+    from verdict_b200.fp8_decoder import Fp8Decoder, synthetic_weights
+    kw = dict(CASES["qwen3"])
+    spec = specs.preset(kw.pop("preset"), layers=1, **kw)
+    here = torch.cuda.current_device()
+    for device in (None, "cuda", torch.device("cuda"), here, f"cuda:{here}"):
+        model = Fp8Decoder(spec, synthetic_weights(spec), device=device)
+        assert model.device == torch.device("cuda", here) == model.embed.device, device
+    with pytest.raises(ValueError):
+        Fp8Decoder(spec, {}, device="cpu")

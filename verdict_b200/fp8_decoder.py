@@ -70,8 +70,12 @@ class Fp8Decoder:
         if spec["head_dim"] not in (128, 256):
             raise ValueError("the attention kernel takes head_dim 128 or 256")
         self.spec = spec
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        dev = self.device
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device or "cuda")
+        if dev.type != "cuda":
+            raise ValueError("Fp8Decoder runs on a CUDA device")
+        if dev.index is None:  # the one that is current now, whichever is when it answers
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.device = dev
 
         def vector(name):
             return weights[name].to(dev, torch.float32).contiguous()
