@@ -155,7 +155,15 @@ VD_API int vdk_fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int
                           char* err, size_t errlen);
 
 /*
- * Failure-path tests only: the same with a limit of its own on every pipeline
+ * How vdk_fp8_linear runs a product on the current device: tokens in a tile (0:
+ * CTA pairs on tiles of 256 x 256), CTAs that share K, and stages of the
+ * shared-memory ring.  Nothing is launched.
+ */
+VD_API int vdk_fp8_linear_plan(int64_t M, int64_t N, int64_t K, int out_dtype, int* tile_rows, int* splits, int* stages,
+                               char* err, size_t errlen);
+
+/*
+ * Failure-path tests only: vdk_fp8_linear with a limit of its own on every pipeline
  * wait, and with each CTA's loads stopping after stall_after blocks of 128
  * columns (-1: never).  Where they stop early, a wait runs out: the kernel
  * ends, status has the wait's code and out is not to be used.

@@ -254,3 +254,9 @@ def test_logprobs_temperature_whose_exponent_factor_overflows_is_refused():
     for t in (3.0e-39, 4.2e-39):
         rc, msg = call("vdk_token_logprobs", FAKE, 20, 2, 20, 0, t, None, 0, 0, None, None, None, None, None)
         assert rc == _abi.VD_EINVAL and "temperature" in msg, (t, rc, msg)
+
+
+def test_a_products_plan_checks_its_arguments():
+    for args in ((4, 4, 128, 3, FAKE, FAKE, FAKE), (0, 4, 128, 0, FAKE, FAKE, FAKE), (4, 4, 128, 0, None, FAKE, FAKE)):
+        err = ctypes.create_string_buffer(512)
+        assert _abi.load().vdk_fp8_linear_plan(*args, err, 512) == _abi.VD_EINVAL and err.value

@@ -98,6 +98,7 @@ SIGNATURES = {
     "vdk_quantize_fp8_weight": (ctypes.c_int, [_P, _I64, _I64, _I64, _INT, _P, _I64, _P, _I64, _P, _STR, _SIZE]),
     "vdk_fp8_linear": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _INT, _P,
                                       _P, _STR, _SIZE]),
+    "vdk_fp8_linear_plan": (ctypes.c_int, [_I64, _I64, _I64, _INT, _P, _P, _P, _STR, _SIZE]),
     "vdk_fp8_linear_stalled": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64,
                                               _INT, _P, _I64, _INT, _P, _STR, _SIZE]),
     "vdk_block_norm": (ctypes.c_int, [_P, _I64, _INT, _P, _I64, _INT, _P, _P, _INT, _I64, _I64, _F32, _F32, _P, _F32,

@@ -198,6 +198,30 @@ void launch_f8_rows(const void* a, int64_t ld_a, const void* w, int64_t ld_w, F8
          f8_map(a, s.M, s.K, ld_a, BN), s, status);
 }
 
+// Which kernel a product runs on.
+struct F8Choice {
+  int bn;           // tokens a tile of fp8_gemm_rows_kernel; 0: CTA pairs
+  F8RowsPlan rows;  // of the former
+};
+
+template <class O>
+F8Choice choose_f8(const F8Shape& s) {
+  if (s.M <= 16) return {16, plan_f8_rows<16, O>(s)};
+  if (s.M <= 32) return {32, plan_f8_rows<32, O>(s)};
+  if (s.M <= 64) return {64, plan_f8_rows<64, O>(s)};
+  // A pair goes through a k-block of a 256 x 256 tile in 0.53 us, a CTA of
+  // the other kernel through one of a 128 x 128 tile in 0.6, but it can split
+  // K, for about four k-blocks' time (bf16, us, pairs / rows: 128 x 6144 x
+  // 4096 19.4 / 14.8, 100 x 4096 x 12288 46.8 / 19.0, 200 x 4096 x 4096 19.1
+  // / 14.8; 256 x 6144 x 4096 19.5 / 21.2, 100 x 24576 x 4096 36.0 / 41.1).
+  const int pairs = sm_count() / 2;
+  const int pair_tiles = ((s.M + 255) / 256) * ((s.N + 255) / 256);
+  const int pair_steps = (pair_tiles + pairs - 1) / pairs * ((s.K + 127) / 128);
+  const F8RowsPlan plan = plan_f8_rows<128, O>(s);
+  const bool rows = plan.steps * 1.1 + 4 < pair_steps && (s.M + 127) / 128 <= 65535;
+  return {rows ? 128 : 0, plan};
+}
+
 // Row-major outputs [rows, cols] with row stride ld, boxes of 32 rows x 128
 // bytes with the 128-byte swizzle; stores past the end are dropped.
 CUtensorMap out_map(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int dtype) {
@@ -318,17 +342,37 @@ extern "C" VD_API int vdk_quantize_fp8_weight(const void* w, int64_t ld_w, int64
   });
 }
 
+static void need_f8_shape(int64_t M, int64_t N, int64_t K, int out_dtype) {
+  need(M >= 0 && N >= 1 && K >= 1, "need M >= 0, N >= 1 and K >= 1");
+  need(M <= (int64_t(1) << 30) && N <= 65535ll * 32 && K <= (int64_t(1) << 30), "a dimension is too large");
+  need(out_dtype >= VDK_FP16 && out_dtype <= VDK_FP32, "out_dtype must be VDK_FP16, VDK_BF16 or VDK_FP32");
+}
+
+extern "C" VD_API int vdk_fp8_linear_plan(int64_t M, int64_t N, int64_t K, int out_dtype, int* tile_rows, int* splits,
+                                          int* stages, char* err, size_t errlen) {
+  return guarded_call(err, errlen, [&] {
+    need_f8_shape(M, N, K, out_dtype);
+    need(M >= 1 && tile_rows && splits && stages, "need rows and somewhere to put the answer");
+    F8Shape s{};
+    s.M = static_cast<int>(M), s.N = static_cast<int>(N), s.K = static_cast<int>(K);
+    by_type(out_dtype, [&](auto tag) {
+      const F8Choice c = choose_f8<decltype(tag)>(s);
+      *tile_rows = c.bn;
+      *splits = c.bn ? c.rows.splits : 1;
+      *stages = c.bn ? c.rows.stages : F8PairConfig::STAGES;
+    });
+  });
+}
+
 static int fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t ld_a_scale, const void* w, int64_t ld_w,
                       const float* w_scale, int64_t ld_w_scale, int64_t M, int64_t N, int64_t K, const float* bias,
                       void* out, int64_t ld_out, int out_dtype, int* status, uint64_t wait_ns, int stall_after,
                       void* stream, char* err, size_t errlen) {
   return guarded_call(err, errlen, [&] {
-    need(M >= 0 && N >= 1 && K >= 1, "need M >= 0, N >= 1 and K >= 1");
-    need(M <= (int64_t(1) << 30) && N <= 65535ll * 32 && K <= (int64_t(1) << 30), "a dimension is too large");
+    need_f8_shape(M, N, K, out_dtype);
     const int64_t kb = (K + 127) / 128;
     need(ld_a >= K && ld_w >= K && ld_out >= N && ld_a_scale >= kb && ld_w_scale >= kb,
          "a row stride is smaller than its row");
-    need(out_dtype >= VDK_FP16 && out_dtype <= VDK_FP32, "out_dtype must be VDK_FP16, VDK_BF16 or VDK_FP32");
     if (M == 0) return;
     need(a && w && a_scale && w_scale && out, "null buffer");
     need(aligned16(a) && ld_a % 16 == 0 && aligned16(w) && ld_w % 16 == 0,
@@ -358,24 +402,14 @@ static int fp8_linear(const void* a, int64_t ld_a, const float* a_scale, int64_t
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     by_type(out_dtype, [&](auto tag) {
       using O = decltype(tag);
-      auto rows = [&](auto bn) {
-        constexpr int BN = decltype(bn)::value;
-        launch_f8_rows<BN, O>(a, ld_a, w, ld_w, s, plan_f8_rows<BN, O>(s), status, st);
-      };
-      if (M <= 16) return rows(std::integral_constant<int, 16>());
-      if (M <= 32) return rows(std::integral_constant<int, 32>());
-      if (M <= 64) return rows(std::integral_constant<int, 64>());
-      // A pair goes through a k-block of a 256 x 256 tile in 0.53 us, a CTA of
-      // the other kernel through one of a 128 x 128 tile in 0.6, but it can split
-      // K, for about four k-blocks' time (bf16, us, pairs / rows: 128 x 6144 x
-      // 4096 19.4 / 14.8, 100 x 4096 x 12288 46.8 / 19.0, 200 x 4096 x 4096 19.1
-      // / 14.8; 256 x 6144 x 4096 19.5 / 21.2, 100 x 24576 x 4096 36.0 / 41.1).
-      const int pairs = sm_count() / 2;
-      const int pair_tiles = ((s.M + 255) / 256) * ((s.N + 255) / 256);
-      const int pair_steps = (pair_tiles + pairs - 1) / pairs * ((s.K + 127) / 128);
-      const F8RowsPlan plan = plan_f8_rows<128, O>(s);
-      if (plan.steps * 1.1 + 4 < pair_steps && (M + 127) / 128 <= 65535) launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, plan, status, st);
-      else launch_f8_pair<O>(a, ld_a, w, ld_w, s, out_dtype, status, st);
+      const F8Choice c = choose_f8<O>(s);
+      switch (c.bn) {
+        case 16: return launch_f8_rows<16, O>(a, ld_a, w, ld_w, s, c.rows, status, st);
+        case 32: return launch_f8_rows<32, O>(a, ld_a, w, ld_w, s, c.rows, status, st);
+        case 64: return launch_f8_rows<64, O>(a, ld_a, w, ld_w, s, c.rows, status, st);
+        case 128: return launch_f8_rows<128, O>(a, ld_a, w, ld_w, s, c.rows, status, st);
+        default: return launch_f8_pair<O>(a, ld_a, w, ld_w, s, out_dtype, status, st);
+      }
     });
   });
 }
