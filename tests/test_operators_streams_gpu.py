@@ -89,3 +89,32 @@ def test_a_graph_reads_its_inputs_when_it_is_replayed():
     side.synchronize()
     assert all(same(got, want)), same(got, want)
     ops.check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 4096, 512), (100, 4096, 2048), (600, 4096, 512)])
+def test_a_product_reads_what_the_product_before_it_wrote(m, n, k):
+    """Each of these kernels is set up while the two before it still run.  A buffer that the first reads as its bias, the
+    second writes as its output and the third reads as its bias again must not come out of a cache."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    a = ops.quantize_fp8(torch.randn(m, k, generator=g, device="cuda"))
+    w = ops.quantize_fp8_weight(torch.randn(n, k, generator=g, device="cuda") * k ** -0.5)
+    one = ops.quantize_fp8(torch.randn(1, k, generator=g, device="cuda"))
+    start = torch.randn(n, generator=g, device="cuda")
+
+    def chain(wait):
+        bias, out = start.clone(), torch.empty(m, n, device="cuda")
+        results = []
+        for _ in range(20):
+            results.append(ops.fp8_linear(*a, *w, bias=bias, out_dtype=torch.float32))   # reads the bias
+            wait()
+            ops.fp8_linear(*one, *w, out_dtype=torch.float32, out=bias.view(1, n))        # writes it
+            wait()
+            ops.fp8_linear(*a, *w, bias=bias, out_dtype=torch.float32, out=out)           # reads it again
+            wait()
+            results.append(out.clone())
+            bias.copy_(start)
+        return results
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        assert all(same(chain(lambda: None), want))

@@ -9,6 +9,10 @@
 // times its scale, to fp32 sums that stay in registers over the whole of K.
 // Several TMEM accumulators keep the MMAs ahead of the drain.
 //
+// Scales and bias are read by plain loads: these kernels are set up while the
+// ones before them still write, and the read-only path is for memory that no one
+// writes while a kernel lives.
+//
 // Two kernels: fp8_gemm_pair_kernel (CTA pairs, 256 x 256 tiles) for many
 // rows, fp8_gemm_rows_kernel (below) for few.
 #pragma once
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
       for (int i = 0; i < PER; ++i) {
         const int e = i * DRAIN + t;
         const int tok = m0 + e / Cfg::SCALE_KB, kb = base + e % Cfg::SCALE_KB;
-        next[i] = tok < s.M && kb < kb1 ? __ldg(s.sa + tok * s.ld_sa + kb) * __ldg(sw + kb) : 0.0f;
+        next[i] = tok < s.M && kb < kb1 ? s.sa[tok * s.ld_sa + kb] * sw[kb] : 0.0f;
       }
     };
     auto put = [&](int chunk) {
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
   if (s.splits == 1) {
     if (warp >= 2 && n < s.N) {
       const int col0 = ((warp - 2) >> 2) * COLS;
-      const float bias = s.bias ? __ldg(s.bias + n) : 0.0f;
+      const float bias = s.bias ? s.bias[n] : 0.0f;
       O* o = out + static_cast<int64_t>(m0 + col0) * s.ld_out + n;
 #pragma unroll
       for (int j = 0; j < COLS; ++j)
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(F8RowsConfig<BN>::THREADS, F8RowsConfig<BN>::C
     __syncwarp();
     cluster_sync_all();  // the sums have arrived
     if (warp >= 2 && n < s.N) {
-      const float bias = s.bias ? __ldg(s.bias + n) : 0.0f;
+      const float bias = s.bias ? s.bias[n] : 0.0f;
       const int first = part * share;
       const int count = min(share, s.M - m0 - first);
       const float4* sums = reinterpret_cast<const float4*>(sSum) + row;
@@ -629,12 +633,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
       // Scales are loaded two k-blocks ahead.
-      float a1 = __ldg(sa), w1 = __ldg(sw);
-      float a2 = kblocks > 1 ? __ldg(sa + 1) : 0.0f, w2 = kblocks > 1 ? __ldg(sw + 1) : 0.0f;
+      float a1 = sa[0], w1 = sw[0];
+      float a2 = kblocks > 1 ? sa[1] : 0.0f, w2 = kblocks > 1 ? sw[1] : 0.0f;
       for (int kb = 0; kb < kblocks; ++kb) {
         const float f = a1 * w1;
         a1 = a2, w1 = w2;
-        if (kb + 2 < kblocks) a2 = __ldg(sa + kb + 2), w2 = __ldg(sw + kb + 2);
+        if (kb + 2 < kblocks) a2 = sa[kb + 2], w2 = sw[kb + 2];
         ok = __all_sync(0xffffffffu, f8_wait(&acc_full[buf], buf_phase, abort_flag, err, kErrTimeoutAccFull, s.wait_ns));
         if (!ok) break;
         tc_fence_after();
@@ -662,7 +666,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
           const float4* b = reinterpret_cast<const float4*>(s.bias + col0);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float4 v = __ldg(b + j);
+            const float4 v = b[j];
             acc[2 * j] = __fadd2_rn(acc[2 * j], make_float2(v.x, v.y));
             acc[2 * j + 1] = __fadd2_rn(acc[2 * j + 1], make_float2(v.z, v.w));
           }
@@ -670,8 +674,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
             const int col = col0 + 2 * j;
-            if (col < s.N) acc[j].x += __ldg(s.bias + col);
-            if (col + 1 < s.N) acc[j].y += __ldg(s.bias + col + 1);
+            if (col < s.N) acc[j].x += s.bias[col];
+            if (col + 1 < s.N) acc[j].y += s.bias[col + 1];
           }
         }
       }
