@@ -427,10 +427,11 @@ extern "C" VD_API int vdk_fp8_linear_stalled(const void* a, int64_t ld_a, const 
                                              int64_t M, int64_t N, int64_t K, const float* bias, void* out,
                                              int64_t ld_out, int out_dtype, int* status, int64_t wait_limit_us,
                                              int stall_after, void* stream, char* err, size_t errlen) {
-  if (wait_limit_us < 1 || wait_limit_us > 2000000 || stall_after < -1) {
-    put_err(err, errlen, "need 1 <= wait_limit_us <= 2e6 and stall_after >= -1");
-    return VD_EINVAL;
-  }
+  const int rc = guarded_call(err, errlen, [&] {
+    need(wait_limit_us >= 1 && wait_limit_us <= 2000000 && stall_after >= -1,
+         "need 1 <= wait_limit_us <= 2e6 and stall_after >= -1");
+  });
+  if (rc != VD_OK) return rc;
   return fp8_linear(a, ld_a, a_scale, ld_a_scale, w, ld_w, w_scale, ld_w_scale, M, N, K, bias, out, ld_out, out_dtype,
                     status, static_cast<uint64_t>(wait_limit_us) * 1000, stall_after, stream, err, errlen);
 }
