@@ -140,8 +140,8 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
 // A drain thread owns a weight row.  The scales a[token] * w of 8 or 16
 // k-blocks at a time lie in shared memory and are read four tokens at once.
 //
-// bf16, device time: 1 x 6144 x 4096 6.7 us (floor 3.8: the weights' 25 MB),
-// 16 x 24576 x 4096 20.5 us (4.9 TB/s), 37 x 4096 x 12288 15.8 us (floor 7.8;
+// bf16, device time: 1 x 6144 x 4096 6.5 us (floor 3.8: the weights' 25 MB),
+// 16 x 24576 x 4096 20.5 us (4.9 TB/s), 37 x 4096 x 12288 16.2 us (floor 7.8;
 // while it streams 5.5 TB/s, the rest is the first loads' latency and the join).
 // ---------------------------------------------------------------------------
 template <int BN>

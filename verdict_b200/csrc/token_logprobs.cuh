@@ -21,6 +21,12 @@
 // Few rows: a cluster of up to eight CTAs shares a row; each pushes its sums
 // and candidates to the first through distributed shared memory.
 //
+// Accuracy: sums are fp32 and the exponentials ex2.approx (1.4e-7 off at most,
+// 5e-8 low on average), of arguments rounded once more by the factor log2(e) /
+// temperature.  All of it stays below the rounding of fp32 outputs of this size:
+// 1.1e-7 relative on a large batch, where exp of an fp32 difference gives 5e-8
+// with more instructions an entry, which are what the batch is bound by.
+//
 // 1024 x 256000 bf16, 8 alternatives: 136 us, 3.9 TB/s, 0.59 of the measured
 // copy rate.  The logits alone are 80 us; the rest is arithmetic (issue slots
 // 61 %, special-function unit 49 %: an exp2 an entry) and the 1.7 waves that
