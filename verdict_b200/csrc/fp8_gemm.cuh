@@ -698,7 +698,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
           }
           *reinterpret_cast<uint4*>(stage_out + lane * 128 + ((q ^ (lane & 7)) << 4)) = w;
         }
-        if (s.out_aligned) {
+        // A TMA store writes whole 16-byte units, past the last column of out as
+        // well: only where a unit does not cross it.
+        if (s.out_aligned && (x + CHUNK <= s.N || s.N % (16 / static_cast<int>(sizeof(O))) == 0)) {
           fence_proxy_async_smem_gemm();
           __syncwarp();
           if (lane == 0) {
@@ -707,7 +709,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8PairConfig::THREAD
           }
           continue;
         }
-        // Rows of out that TMA cannot address: row by row, lanes along columns.
+        // What TMA cannot store: row by row, lanes along columns.
         __syncwarp();
         constexpr int EL = 4 / sizeof(O);  // outputs in a lane's four bytes
         const int left = s.N - x - lane * EL, rows = min(32, s.M - row0);

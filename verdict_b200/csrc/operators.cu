@@ -223,7 +223,8 @@ F8Choice choose_f8(const F8Shape& s) {
 }
 
 // Row-major outputs [rows, cols] with row stride ld, boxes of 32 rows x 128
-// bytes with the 128-byte swizzle; stores past the end are dropped.
+// bytes with the 128-byte swizzle; stores past the end are dropped, columns in
+// units of 16 bytes.
 CUtensorMap out_map(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int dtype) {
   CUtensorMap m;
   const int es = elem_bytes(dtype);
