@@ -118,3 +118,32 @@ def test_a_product_reads_what_the_product_before_it_wrote(m, n, k):
     want = chain(torch.cuda.synchronize)
     for _ in range(5):
         assert all(same(chain(lambda: None), want))
+
+
+def test_products_of_every_kind_on_several_streams_at_once():
+    """CTAs of different products meet on an SM and share its tensor memory; the answers are those of one at a time."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    work = []
+    for m, n, k in ((3, 512, 32768), (16, 24576, 1024), (30, 512, 32768), (50, 4096, 12288), (64, 20000, 1024),
+                    (100, 4096, 12288), (100, 3000, 300), (600, 2048, 4096)):
+        a = ops.quantize_fp8(torch.randn(m, k, generator=g, device="cuda"))
+        w = ops.quantize_fp8_weight(torch.randn(n, k, generator=g, device="cuda") * k ** -0.5)
+        work.append((a, w))
+    logits = torch.randn(4, 152064, generator=g, device="cuda")
+    run = lambda i: ops.fp8_linear(*work[i][0], *work[i][1])  # noqa: E731
+    want = [run(i) for i in range(len(work))]
+    want_lp = ops.token_logprobs(logits, top=5)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got, got_lp = [], []
+    for rounds in range(12):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                for j in range(len(work)):
+                    i = (j * (2 * s + 1) + rounds + s) % len(work)
+                    got.append((i, run(i)))
+                got_lp.append(ops.token_logprobs(logits, top=5))
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert all(torch.equal(t, want[i]) for i, t in got)
+    assert all(torch.equal(a, b) for r in got_lp for a, b in zip(r[1:], want_lp[1:]))
