@@ -552,6 +552,9 @@ extern "C" VD_API int vdk_rotary_turns(double theta, int rotary_dim, int scaling
     // A turn in 64 bits wants more than a double's 53 at every step up to it:
     // the position multiplies what is lost here.
     using real = long double;
+#ifndef __CUDA_ARCH__
+    static_assert(std::numeric_limits<real>::digits >= 64, "the turns need 64 bits");
+#endif
     const real two_pi = 6.283185307179586476925286766559005768L;
     const int half = rotary_dim / 2;
     const double d = rotary_dim;
@@ -694,7 +697,8 @@ extern "C" VD_API int vdk_token_logprobs(const void* logits, int64_t ld, int64_t
     need(rows >= 0 && rows <= kMaxInt / 8 && vocab >= 1 && vocab <= kMaxInt - 65536,
          "need 0 <= rows < 2^28 and 1 <= vocab < 2^31 - 65536");
     need(ld >= vocab, "a row stride is smaller than its row");
-    need(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(static_cast<float>(1.4426950408889634 / temperature)),
+    need(std::isfinite(temperature) && temperature > 0.0f &&
+             std::isfinite(static_cast<float>(1.4426950408889634 / temperature)),
          "temperature must be positive (at least 4.3e-39)");
     need(top >= 0 && top <= VDK_LOGPROBS_MAX_TOP, "top must be from 0 to VDK_LOGPROBS_MAX_TOP");
     need(n_targets >= 0 && n_targets <= kMaxInt, "n_targets must not be negative");
